@@ -962,7 +962,10 @@ void device_errors_to_host(Tensor host) {
 
 }  // namespace
 
+void bind_serving(py::module_& m);  // bindings_serving.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_serving(m);
   m.doc() = "sm_100a kernels: tcgen05 GEMMs with fused epilogues, flash attention, norms, optimizer, collectives";
   m.def("linear_fwd", &linear_fwd, py::arg("x"), py::arg("w"), py::arg("out"), py::arg("residual") = py::none(),
         py::arg("bn") = 0);

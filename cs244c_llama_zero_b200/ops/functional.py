@@ -12,7 +12,7 @@ fallback on this path.
 from __future__ import annotations
 
 import math
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -261,6 +261,112 @@ def attention_backward(qkv: torch.Tensor, out: torch.Tensor, dout: torch.Tensor,
     _ext().attention_bwd(qkv, heads * head_dim, (heads + kv_heads) * head_dim, out, dout.contiguous(), lse, delta,
                          dq_acc, dqkv, cos, sin, batch, seq, heads, kv_heads, head_dim, 1.0 / math.sqrt(head_dim),
                          True)
+
+
+# ------------------------------------------------------------------------------ paged key/value cache
+class KVPages(NamedTuple):
+    """One layer's paged key/value cache.
+
+    ``k`` and ``v`` are pools of pages ``[n_pages, kv_heads, page_size, head_dim]`` (contiguous, page_size
+    16, 32, 64 or 128) in bfloat16, or in 8 bits (float8_e4m3fn or int8) with one float32 scale per token
+    and head in ``k_scale`` / ``v_scale`` ``[n_pages, kv_heads, page_size]``: a row ``x`` is stored as
+    ``scale = max|x| / M`` and ``code = round(x * M / max|x|)`` with M = 448 (e4m3) or 127 (int8).  A row
+    with an infinity or a NaN gets the scale NaN and reads back as NaN.
+
+    A batch of sequences over such pages is described by ``block_table`` (int32 ``[batch, pages]``: token t
+    of sequence b lies in page ``block_table[b, t // page_size]``), ``kv_lens`` (int32 ``[batch]``: cached
+    tokens, the new ones included) and ``q_starts`` (int32 ``[batch + 1]``: rows ``q_starts[b]`` to
+    ``q_starts[b + 1]`` of the token tensors are the last tokens of sequence b; ``None``: one row each).
+    All three live on the device and are read by the kernels only, so calls can be captured in a CUDA
+    graph.  Values that do not fit (a length past the table, rows outside the tensor, a page that does not
+    exist) are skipped and recorded: ``ops.check_device_errors()`` raises for them.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+
+def _no_backward(name: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
+
+
+def kv_cache_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
+                   kv_lens: torch.Tensor, q_starts: Optional[torch.Tensor] = None) -> None:
+    """Write the new tokens' keys and values (bf16 ``[tokens, kv_heads, head_dim]``, any row strides that
+    are multiples of 8) to their places in the cache, quantising them if the pages are 8-bit.  The pages
+    that take new tokens must belong to one sequence each.  Rows of no sequence are ignored."""
+    _no_backward("kv_cache_write", k, v)
+    _ext().kv_cache_write(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, block_table, kv_lens, q_starts)
+
+
+def kv_cache_read(pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                  q_starts: Optional[torch.Tensor] = None, total: Optional[int] = None,
+                  dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The last tokens of every sequence out of the cache, as ``[total, kv_heads, head_dim]`` keys and
+    values (bfloat16 or float32).  ``total`` is the number of rows (``q_starts[-1]``; default: one per
+    sequence).  A row before its sequence's first token is zero; rows of no sequence are not written."""
+    if total is None:
+        if q_starts is not None:
+            raise ValueError("kv_cache_read: total (the number of rows) is needed with q_starts")
+        total = block_table.shape[0]
+    shape = (total, pages.k.shape[1], pages.k.shape[3])
+    k = torch.empty(shape, dtype=dtype, device=pages.k.device)
+    v = torch.empty(shape, dtype=dtype, device=pages.k.device)
+    _ext().kv_cache_read(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, block_table, kv_lens, q_starts)
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                    q_starts: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of the new tokens ``q`` (bf16 ``[tokens, heads, head_dim]``) over the cache.
+
+    Row i of a sequence's q_len new tokens stands at position ``kv_len - q_len + i`` and sees the cached
+    tokens up to and including that position (their keys and values must have been written); a row whose
+    position is negative sees nothing and gives zeros.  Query head h reads kv head
+    ``h // (heads / kv_heads)``; scores are scaled by ``scale`` (default ``head_dim ** -0.5``).
+    ``max_q_len`` bounds the new tokens of any sequence and is required with ``q_starts``.  ``out`` (default:
+    a new tensor) must not share memory with ``q``; rows of no sequence are not written.  Whatever lies in
+    the pages behind a sequence's end is not looked at; a NaN among the cached tokens of a sequence makes
+    its rows NaN."""
+    _no_backward("paged_attention", q)
+    if max_q_len is None:
+        if q_starts is not None:
+            raise ValueError("paged_attention: max_q_len is needed with q_starts")
+        max_q_len = 1
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _ext().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, out, block_table, kv_lens, q_starts,
+                           max_q_len, q.shape[-1] ** -0.5 if scale is None else scale)
+    return out
+
+
+# ------------------------------------------------------------------------------ logits
+def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
+                  history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                  repetition_penalty: Optional[torch.Tensor] = None,
+                  frequency_penalty: Optional[torch.Tensor] = None,
+                  presence_penalty: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Next-token logits ``[batch, vocab]`` (bf16, fp16 or fp32) with penalties, biases and a grammar mask.
+
+    ``history`` (int64 ``[batch, length]``, the first ``history_lens`` (int32) of each row) holds the tokens
+    so far, the first ``prompt_lens`` (int32, default 0) of them the prompt.  With float32 penalties per
+    row, in this order: a token that occurs in the history has its logit divided by ``repetition_penalty``
+    if positive, else multiplied by it; ``frequency_penalty * n + presence_penalty * (n > 0)`` is
+    subtracted for a token that was generated n times; ``bias`` (float32 ``[vocab]`` or ``[batch, vocab]``)
+    is added; tokens whose bit in ``allowed`` (int32 ``[ceil(vocab / 32)]`` or one row each, token t at bit
+    ``t % 32`` of word ``t // 32``) is 0 become ``-inf``.  Computed in fp32.  ``out`` may be ``logits``.
+    A token id outside the vocabulary is skipped and recorded (``ops.check_device_errors()``)."""
+    _no_backward("adjust_logits", logits)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _ext().adjust_logits(logits, out, history, history_lens, prompt_lens, repetition_penalty, frequency_penalty,
+                         presence_penalty, bias, allowed)
+    return out
 
 
 # ------------------------------------------------------------------------------ transformer block
