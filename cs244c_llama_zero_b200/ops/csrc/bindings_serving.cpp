@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "paged.h"
+#include "paged_sched.cuh"
 
 namespace {
 
@@ -201,7 +202,58 @@ void paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, std::optional<Ten
   p.heads = (int)heads;
   p.group = (int)(heads / pool.kv_heads);
   p.scale = (float)scale;
-  b200::paged_attention(p, cur_stream());
+  Tensor workspace;  // from PyTorch's allocator: reused in stream order, private to a graph that captures the call
+  b200::paged_attention(
+      p,
+      [&](size_t bytes) {
+        workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        return workspace.data_ptr();
+      },
+      cur_stream());
+}
+
+// Host-only view of how the attention kernels divide their work (CPU tensors, no GPU needed): per block and
+// item (block, sequence, kv head, tile, first unit in the item, end unit, units of the item).
+std::vector<std::vector<int64_t>> paged_schedule(Tensor starts, Tensor lens, int64_t max_tokens, int64_t total_q,
+                                                 int64_t max_q, int64_t kv_heads, int64_t tile_tokens,
+                                                 int64_t unit_log2, int64_t grid) {
+  TORCH_CHECK(!lens.is_cuda() && !starts.is_cuda() && lens.scalar_type() == at::kInt &&
+                  starts.scalar_type() == at::kInt && lens.is_contiguous() && starts.is_contiguous() &&
+                  starts.numel() == lens.numel() + 1,
+              "paged_schedule: contiguous int32 CPU tensors required");
+  b200::PagedSeqs s{};
+  s.kv_lens = lens.data_ptr<int>();
+  s.q_starts = starts.data_ptr<int>();
+  s.batch = (int)lens.numel();
+  s.max_pages = (int)max_tokens;
+  s.total_q = (int)total_q;
+  s.max_q = (int)max_q;
+  const b200::PagedShape shape{(int)tile_tokens, (int)unit_log2, (int)kv_heads};
+  std::vector<std::vector<int64_t>> out;
+  long long total = 0;
+  std::vector<long long> base;
+  for (int b = 0; b < s.batch; ++b) {
+    base.push_back(total);
+    total += b200::head_units(b200::seq_info(s, b), shape) * kv_heads;
+  }
+  const long long blocks = std::min<long long>(grid, total);
+  for (long long c = 0; c < blocks; ++c) {
+    long long u = b200::range_begin(c, total, blocks);
+    const long long end = b200::range_begin(c + 1, total, blocks);
+    TORCH_CHECK(b200::block_of_unit(u, total, blocks) == c && b200::block_of_unit(end - 1, total, blocks) == c,
+                "paged_schedule: block_of_unit");
+    int b = s.batch - 1;
+    while (base[b] > u || b200::seq_info(s, b).qn == 0) --b;
+    b200::PagedItem it = b200::item_at(s, shape, b, base[b], u);
+    while (true) {
+      const long long stop = std::min(end, it.start + it.n_units);
+      out.push_back({c, it.b, it.kvh, it.rt, u - it.start, stop - it.start, it.n_units});
+      u = stop;
+      if (u == end) break;
+      b200::next_item(it, s, shape);
+    }
+  }
+  return out;
 }
 
 void check_per_row(const std::optional<Tensor>& t, const Tensor& logits, at::ScalarType type, const char* name) {
@@ -294,5 +346,6 @@ void bind_serving(pybind11::module_& m) {
   m.def("kv_cache_write", &kv_cache_write);
   m.def("kv_cache_read", &kv_cache_read);
   m.def("paged_attention", &paged_attention);
+  m.def("paged_schedule", &paged_schedule);
   m.def("adjust_logits", &adjust_logits);
 }

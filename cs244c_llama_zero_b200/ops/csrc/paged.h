@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <functional>
+
 #include "common.cuh"
 
 namespace b200 {
@@ -90,7 +92,10 @@ struct PagedAttnParams {
   float scale;
   DeviceErrors* errs;
 };
-void paged_attention(const PagedAttnParams& p, cudaStream_t s);
+// `alloc` returns device memory of at least the given size (16-byte aligned) that stays valid for the work
+// enqueued on the stream by this call.
+using PagedAlloc = std::function<void*(size_t)>;
+void paged_attention(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
 
 struct LogitsParams {
   const void* logits;  // [batch, vocab], row stride in elements

@@ -133,3 +133,49 @@ def test_bad_logits(F):
     wide = torch.zeros(2, 80)
     with pytest.raises(RuntimeError, match="share memory"):
         F.adjust_logits(wide[:, :40], out=wide[:, 20:60])
+
+
+# ------------------------------------------------------------------------------------------ work division
+@pytest.mark.parametrize("tile_tokens,unit_log2,grid", [(16, 6, 296), (2, 6, 5), (64, 7, 148), (42, 7, 7), (256, 7, 1),
+                                                        (1, 6, 592)])
+@pytest.mark.parametrize("seed", range(4))
+def test_every_unit_is_done_once(F, tile_tokens, unit_log2, grid, seed):
+    """The blocks' ranges cover all units of all items once, in order, and differ by at most one unit."""
+    from cs244c_llama_zero_b200 import ops
+
+    from tests.serving_reference import ragged
+
+    q, kv = ragged(seed, (1, 3, 40, 300)[seed], (1, 200, 90, 3)[seed], (5000, 700, 300, 900)[seed])
+    q[-1] = max(q[-1], 1)
+    kv[0] = 0  # rows that see nothing
+    starts = torch.tensor([sum(q[:i]) for i in range(len(q) + 1)], dtype=torch.int32)
+    lens = torch.tensor(kv, dtype=torch.int32)
+    heads = 3
+    parts = ops.load_extension().paged_schedule(starts, lens, 100_000, sum(q), max(q), heads, tile_tokens, unit_log2,
+                                                grid)
+    want = []
+    for b, (n, t) in enumerate(zip(q, kv)):
+        for h in range(heads):
+            for rt in range(-(-n // tile_tokens)):
+                visible = t - n + min(n, (rt + 1) * tile_tokens)
+                want.append((b, h, rt, max(1, -(-visible // (1 << unit_log2)))))
+    got, sizes = [], {}
+    for block, b, h, rt, u0, u1, units in parts:
+        sizes[block] = sizes.get(block, 0) + u1 - u0
+        assert 0 <= u0 < u1 <= units
+        if u0 == 0:
+            got.append([b, h, rt, 0])
+        assert got[-1][:3] == [b, h, rt] and got[-1][3] == u0
+        got[-1][3] = u1
+    assert [tuple(g) for g in got] == want
+    assert sorted(sizes) == list(range(min(grid, sum(w[3] for w in want))))
+    assert max(sizes.values()) - min(sizes.values()) <= 1
+
+
+def test_bad_sequences_get_no_units(F):
+    from cs244c_llama_zero_b200 import ops
+
+    starts = torch.tensor([0, 2, 1, 4, 9, 10], dtype=torch.int32)  # rows that run backwards, too many, too few
+    lens = torch.tensor([64, 64, 65, 64, -1], dtype=torch.int32)  # 65: past the table
+    parts = ops.load_extension().paged_schedule(starts, lens, 64, 10, 4, 1, 4, 6, 8)
+    assert [p[1:] for p in parts] == [[0, 0, 0, 0, 1, 1]]
