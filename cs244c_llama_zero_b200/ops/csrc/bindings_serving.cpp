@@ -44,7 +44,7 @@ RowStrides check_rows(const Tensor& x, int64_t tokens, int64_t heads, int64_t hd
   TORCH_CHECK(x.scalar_type() == at::kBFloat16, name, " must be bfloat16");
   TORCH_CHECK(x.stride(2) == 1, name, " must have unit stride along head_dim");
   RowStrides s{x.size(0) > 1 ? x.stride(0) : heads * hd, x.size(1) > 1 ? x.stride(1) : hd};
-  TORCH_CHECK(s.t % 8 == 0 && s.h % 8 == 0 && s.t >= 0 && s.h >= 0, name, " strides must be multiples of 8 elements");
+  TORCH_CHECK(s.t % 8 == 0 && s.h % 8 == 0 && s.t > 0 && s.h > 0, name, " strides must be positive multiples of 8 elements");
   if (written)
     TORCH_CHECK(s.h >= hd && (x.size(0) <= 1 || s.t >= (heads - 1) * s.h + hd), name,
                 " must not overlap itself and must be laid out token by token");

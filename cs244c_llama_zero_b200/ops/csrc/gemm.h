@@ -81,6 +81,9 @@ CUtensorMap make_tmap_2d(CUtensorMapDataType dtype, int elem_bytes, const void* 
                          CUtensorMapSwizzle swizzle);
 CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
                               uint32_t box_inner, uint32_t box_outer);
+// 3D bf16 map with 128-byte swizzle (dims {d0, d1, d2}, strides of dimensions 1 and 2 in elements).
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
+                              uint64_t stride2, uint32_t box0, uint32_t box1, uint32_t box2);
 void gemm_launch(const GemmOperands& op, GemmParams p, int epi, bool a_mn, bool b_mn, int bn, cudaStream_t stream);
 // One persistent launch computing two independent GEMMs of a linear layer's backward pass:
 //   problem 0: dX[M0, N0] = dY[M0, K0] @ W[K0, N0]          (A K-major, B MN-major, bf16 store)

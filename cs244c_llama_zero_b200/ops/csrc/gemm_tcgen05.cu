@@ -682,6 +682,22 @@ CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, 
                    CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
+                              uint64_t stride2, uint32_t box0, uint32_t box1, uint32_t box2) {
+  B200_CHECK((reinterpret_cast<uintptr_t>(base) & 15) == 0, "TMA base address must be 16-byte aligned");
+  B200_CHECK(stride1 % 8 == 0 && stride2 % 8 == 0, "TMA strides must be multiples of 16 bytes");
+  CUtensorMap map;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {stride1 * 2, stride2 * 2};
+  cuuint32_t box[3] = {box0, box1, box2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = get_encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  B200_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
+  return map;
+}
+
 // Epilogue output / residual maps: one staging chunk (32 rows x 64 B) per box, 64-byte swizzle.
 static CUtensorMap epi_map_bf16(const void* base, int rows, int cols, int ld) {
   return make_tmap_2d(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, (uint64_t)cols, (uint64_t)rows, (uint64_t)ld, 32, 32,

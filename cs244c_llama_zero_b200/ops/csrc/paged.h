@@ -96,6 +96,8 @@ struct PagedAttnParams {
 // enqueued on the stream by this call.
 using PagedAlloc = std::function<void*(size_t)>;
 void paged_attention(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
+// Its form for more than 16 rows per kv head and sequence (paged_chunk.cu).
+void paged_attention_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
 
 struct LogitsParams {
   const void* logits;  // [batch, vocab], row stride in elements

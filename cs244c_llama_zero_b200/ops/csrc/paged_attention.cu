@@ -19,7 +19,6 @@
 //   before they are rounded to bf16.
 // The running maximum is raised only when a score exceeds it by more than 2^8 (one vote per 16 tokens).
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -584,75 +583,6 @@ void launch_decode(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream
   count_launch(2);
 }
 
-template <int FMT>
-__device__ __forceinline__ float load_code(const void* base, long long idx) {
-  if constexpr (FMT == KV_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[idx]);
-  if constexpr (FMT == KV_E4M3) return (float)reinterpret_cast<const __nv_fp8_e4m3*>(base)[idx];
-  return (float)reinterpret_cast<const int8_t*>(base)[idx];
-}
-
-// One warp per (row, head): lane l holds columns l, l + 32, ...
-template <int FMT, int HD>
-__global__ void __launch_bounds__(256) paged_attn_simple_kernel(PagedAttnParams p) {
-  pdl_wait_and_release();
-  constexpr int N = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= (long long)p.seqs.total_q * p.heads) return;
-  const int t = (int)(w / p.heads), h = (int)(w % p.heads);
-  const int b = seq_of_row(p.seqs, t);
-  if (b < 0) return;
-  const SeqInfo si = seq_info(p.seqs, b);
-  if (!si.ok || t < si.q0 || t >= si.q0 + si.qn) {
-    if (lane == 0) report_error(p.errs, kErrBadIndex, b);
-    return;
-  }
-  const int pos = si.len - si.qn + (t - si.q0);
-  const int kvh = h / p.group;
-  float q[N], o[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = __bfloat162float(p.q[t * p.q_stride_t + h * p.q_stride_h + lane + 32 * i]) * p.scale * kLog2e;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j <= pos; ++j) {
-    const int page = p.seqs.table[(long long)b * p.seqs.table_stride + (j >> p.seqs.page_log2)];
-    if (page < 0 || page >= p.seqs.n_pages) {
-      if (lane == 0) report_error(p.errs, kErrBadIndex, b);
-      continue;
-    }
-    const long long cell = (((long long)page * p.pool.kv_heads + kvh) << p.seqs.page_log2) +
-                           (j & ((1 << p.seqs.page_log2) - 1));
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += q[i] * load_code<FMT>(p.pool.k, cell * HD + lane + 32 * i);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (FMT != KV_BF16) s *= p.pool.k_scale[cell];
-    const float m_new = fmaxf(m, s);
-    const float alpha = m == m_new ? 1.f : exp2f(m - m_new);
-    const float pr = exp2f(s - m_new);
-    const float pv = FMT != KV_BF16 ? pr * p.pool.v_scale[cell] : pr;
-    l = l * alpha + pr;
-    m = m_new;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * alpha + pv * load_code<FMT>(p.pool.v, cell * HD + lane + 32 * i);
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    p.out[t * p.o_stride_t + h * p.o_stride_h + lane + 32 * i] = __float2bfloat16_rn(o[i] * inv);
-}
-
-template <int FMT, int HD>
-void launch_simple(const PagedAttnParams& p, cudaStream_t s) {
-  const long long warps = (long long)p.seqs.total_q * p.heads;
-  launch_k(paged_attn_simple_kernel<FMT, HD>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, 1, p);
-  B200_CUDA_CHECK(cudaGetLastError());
-  count_launch();
-}
-
 template <int FMT, int HD>
 void launch_rows(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
   const long long rows = (long long)p.seqs.max_q * p.group;
@@ -661,7 +591,7 @@ void launch_rows(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t
   else if (rows <= 16)
     launch_decode<FMT, HD, 2>(p, alloc, s);
   else
-    launch_simple<FMT, HD>(p, s);
+    paged_attention_chunk(p, alloc, s);
 }
 
 template <int FMT>

@@ -1,0 +1,685 @@
+// Attention of chunks of new tokens over a paged key/value cache, on the 5th-generation tensor cores.
+//
+// The heads that share a kv head are packed with the tokens: a tile's 128 rows are 128 / group consecutive
+// tokens times the group's heads, so K and V are staged once for the whole group.  An item is two such tiles
+// (A and B) of one sequence and kv head; units are 128 cached tokens; a block per SM streams an equal share of
+// all units (paged_sched.cuh), so that one long sequence fills the device as well as many short ones.
+//
+// Warpgroups (the first hands registers to the others with setmaxnreg):
+//   0: warp 0 loads Q (TMA: box of 64 columns x group heads x tokens) and, for bf16 pages, K and V (TMA: one box
+//      per page and 64 columns); warp 1 issues the MMAs; warp 2 zeroes V's rows behind the last visible token.
+//   1, 2: softmax of tile A and B, one thread per row, as in the training forward kernel: scores from tensor
+//      memory, probabilities back into the same columns as the A operand of the PV product, lazy rescaling of O.
+//   3 (8-bit pages only): expands codes into the shared-memory tiles as bf16 (code * scale, rounded once: half a
+//      step of 2^-8 relative, as for unquantised bf16 keys and values).
+// MMA order: S_A(0) S_B(0) | PV_A(j) S_A(j+1) PV_B(j) S_B(j+1) | ...
+//
+// Masking is by selection (a masked score becomes -inf whatever K holds), and V's rows behind the last visible
+// token are zeroed in shared memory before they meet the zero probabilities: what lies in a page behind a
+// sequence's end, a NaN included, has no influence.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "gemm.h"
+#include "kernels.h"
+#include "paged.h"
+#include "paged_sched.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr int kItemRows = 256;
+
+template <int FMT, int HD>
+struct ChunkCfg {
+  static constexpr bool QUANT = FMT != KV_BF16;
+  static constexpr int THREADS = QUANT ? 512 : 384;
+  static constexpr int LAUNCH_REGS = QUANT ? 128 : 168;
+  static constexpr int KB = HD / 64;
+  static constexpr int TILE_BYTES = 128 * HD * 2;
+  static constexpr int STAGES = (HD == 64) ? 3 : 2;
+  static constexpr int Q_BUFS = (HD == 64) ? 2 : 1;
+  static constexpr int REGS_LOW = QUANT ? 48 : 88;
+  static constexpr int REGS_CONV = QUANT ? 80 : 0;
+  static constexpr int REGS_HIGH = QUANT ? 192 : 208;
+  static constexpr int REGS_NEEDED = 128 * REGS_LOW + 256 * REGS_HIGH + 128 * REGS_CONV;
+  static_assert(REGS_NEEDED <= THREADS * LAUNCH_REGS, "register split over budget");
+  // hd 64: row sums from the tensor cores, by a block of ones behind V (see the training forward kernel)
+  static constexpr bool ONES = (HD == 64);
+  static constexpr int O_COLS = ONES ? HD + 16 : HD;
+  static constexpr int STAGE_BYTES = (ONES ? 3 : 2) * TILE_BYTES;
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = Q_BUFS * 2 * TILE_BYTES;
+  static constexpr int BAR_OFF = KV_OFF + STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
+  static_assert(SMEM_BYTES + 512 <= 232448, "shared memory exceeds 227 KB");
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int T_S = 0;
+  static constexpr int T_O = 256;
+  static_assert(T_O + 2 * O_COLS <= TMEM_COLS, "tensor memory");
+};
+
+// One block's walk over its items, the same in every role.
+struct ChunkWalk {
+  PagedItem it;
+  long long u, u_end;
+  int j0, j1;      // units of the item in this block's range
+  int n_tiles;     // 1: the item has rows in tile A only
+  int visible;     // cached tokens that its last row sees
+  bool whole;
+};
+__device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh) {
+  const long long end = w.it.start + w.it.n_units;
+  w.j0 = (int)(w.u - w.it.start);
+  w.j1 = (int)((w.u_end < end ? w.u_end : end) - w.it.start);
+  w.whole = w.j0 == 0 && w.j1 == w.it.n_units;
+  w.n_tiles = w.it.seq.qn - w.it.rt * sh.tile_tokens > sh.tile_tokens / 2 ? 2 : 1;
+  w.visible = item_visible(w.it.seq, w.it.rt, sh.tile_tokens);
+}
+__device__ __forceinline__ bool leave_item(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh) {
+  w.u += w.j1 - w.j0;
+  if (w.u == w.u_end) return false;
+  next_item(w.it, s, sh);
+  enter_item(w, sh);
+  return true;
+}
+
+// 16 codes times their row's scale as 16 bf16.
+template <int FMT>
+__device__ __forceinline__ void expand16(const uint4& q, float scale, uint4 (&out)[2]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[4];
+    if constexpr (FMT == KV_E4M3) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[i] >> (16 * h)) & 0xFFFFu), __NV_E4M3);
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+        f[2 * h] = v.x;
+        f[2 * h + 1] = v.y;
+      }
+    } else {
+      // code + 128 as the low bits of 2^23, exactly; then 2^23 + 128 is taken off
+      const uint32_t b = w[i] ^ 0x80808080u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7440 + e)) - 8388736.0f;
+    }
+    r[2 * i] = pack_bf16(f[0] * scale, f[1] * scale);
+    r[2 * i + 1] = pack_bf16(f[2] * scale, f[3] * scale);
+  }
+  out[0] = make_uint4(r[0], r[1], r[2], r[3]);
+  out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnParams p,
+                       PagedShape shape, PagedWorkspace ws) {
+  using C = ChunkCfg<FMT, HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = q_full + C::Q_BUFS;
+  uint64_t* kv_full = q_empty + C::Q_BUFS;
+  uint64_t* kv_empty = kv_full + C::STAGES;
+  uint64_t* s_full = kv_empty + C::STAGES;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* o_free = o_done + 2;
+  uint64_t* v_zeroed = o_free + 2;  // per stage (bf16): V's rows behind the last visible token are zeros
+  uint64_t* v_raw = v_zeroed + C::STAGES;  // per stage (bf16): V of such a tile has arrived
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_raw + C::STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::Q_BUFS; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&kv_full[s], C::QUANT ? 4 : 1);
+      mbar_init(&kv_empty[s], 1);
+      mbar_init(&v_zeroed[s], 1);
+      mbar_init(&v_raw[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+      mbar_init(&o_free[t], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if constexpr (C::ONES) {
+    for (int st = 0; st < C::STAGES; ++st) {
+      uint4* ones = reinterpret_cast<uint4*>(smem + C::KV_OFF + st * C::STAGE_BYTES + 2 * C::TILE_BYTES);
+      for (int i = threadIdx.x; i < C::TILE_BYTES / 16; i += C::THREADS)
+        ones[i] = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait_and_release();
+
+  const PagedRange range = find_range<C::THREADS>(p.seqs, shape, p.errs);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    ws.total[0] = range.total;
+    ws.total[1] = range.blocks;
+  }
+  const bool busy = (int)blockIdx.x < range.blocks;
+  ChunkWalk w;
+  if (busy) {
+    w.u = range_begin(blockIdx.x, range.total, range.blocks);
+    w.u_end = range_begin(blockIdx.x + 1, range.total, range.blocks);
+    w.it = item_at(p.seqs, shape, range.b, range.base, w.u);
+    enter_item(w, shape);
+    if (threadIdx.x == 0) ws.records[blockIdx.x] = {w.it.start, w.it.n_units, w.it.b, w.it.kvh, w.it.rt};
+  }
+  const int tile_tokens = shape.tile_tokens / 2;  // of one tile
+  const int page_log2 = p.seqs.page_log2;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_LOW));
+    if (busy && warp == 0 && lane == 0) {
+      tma_prefetch_desc(&tm_q);
+      int g = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int qs = k % C::Q_BUFS;
+        if (k >= C::Q_BUFS &&
+            !mbar_wait_bounded(&q_empty[qs], ((k / C::Q_BUFS) - 1) & 1, abort_flag, p.errs, kErrAttnWait, 10))
+          break;
+        uint8_t* qbase = smem + C::Q_OFF + qs * 2 * C::TILE_BYTES;
+        mbar_expect_tx(&q_full[qs], w.n_tiles * C::KB * tile_tokens * p.group * 128);
+        for (int t = 0; t < w.n_tiles; ++t)
+#pragma unroll
+          for (int kb = 0; kb < C::KB; ++kb)
+            tma_load_3d(qbase + t * C::TILE_BYTES + kb * 16384, &tm_q, &q_full[qs], 64 * kb, w.it.kvh * p.group,
+                        w.it.seq.q0 + w.it.rt * shape.tile_tokens + t * tile_tokens);
+        if constexpr (!C::QUANT) {
+          const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
+          const int page_size = 1 << page_log2;
+          for (int j = w.j0; j < w.j1; ++j, ++g) {
+            const int st = g % C::STAGES;
+            if (!mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0)) {
+              ok = false;
+              break;
+            }
+            uint8_t* ks = smem + C::KV_OFF + st * C::STAGE_BYTES;
+            uint8_t* vs = ks + C::TILE_BYTES;
+            const int n_pages = min(128 >> page_log2, max(0, (w.visible - j * 128 + page_size - 1) >> page_log2));
+            // a tile that the sequence ends in gets V on a barrier of its own: warp 2 zeroes its tail first
+            const bool tail = (j + 1) * 128 > w.visible;
+            uint64_t* v_bar = tail ? &v_raw[st] : &kv_full[st];
+            const int bytes = n_pages * page_size * HD * 2;
+            mbar_expect_tx(&kv_full[st], tail ? bytes : 2 * bytes);
+            if (tail) mbar_expect_tx(&v_raw[st], bytes);
+            for (int i = 0; i < n_pages; ++i) {
+              int page = table[((j * 128) >> page_log2) + i];
+              if (page < 0 || page >= p.seqs.n_pages) {
+                report_error(p.errs, kErrBadIndex, w.it.b);
+                page = p.seqs.n_pages;  // behind the tensor: the copy fills zeros
+              }
+              const int row = (int)(min((long long)page * shape.kv_heads + w.it.kvh,
+                                        (long long)p.seqs.n_pages * shape.kv_heads)
+                                    << page_log2);
+              const int at = i * page_size * 128;
+#pragma unroll
+              for (int kb = 0; kb < C::KB; ++kb) {
+                tma_load_2d(ks + kb * 16384 + at, &tm_k, &kv_full[st], 64 * kb, row);
+                tma_load_2d(vs + kb * 16384 + at, &tm_v, v_bar, 64 * kb, row);
+              }
+            }
+          }
+        }
+        if (!ok || !leave_item(w, p.seqs, shape)) break;
+      }
+    } else if (busy && warp == 1 && lane == 0) {
+      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false);
+      constexpr uint32_t IDESC_O = idesc_bf16_f32(128, C::O_COLS, false, true);
+      int g = 0;
+      uint32_t zeroed_parity = 0;  // bit per stage
+      int pn[2] = {0, 0}, on[2] = {0, 0};
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int qs = k % C::Q_BUFS;
+        const uint32_t q_addr = smem_u32(smem + C::Q_OFF + qs * 2 * C::TILE_BYTES);
+        if (!mbar_wait_bounded(&q_full[qs], (k / C::Q_BUFS) & 1, abort_flag, p.errs, kErrAttnWait, 2)) break;
+        auto issue_s = [&](int t, int st) {
+          const uint64_t dq = smem_desc_sw128(q_addr + t * C::TILE_BYTES, 16, 1024);
+          const uint64_t dk = smem_desc_sw128(smem_u32(smem + C::KV_OFF + st * C::STAGE_BYTES), 16, 1024);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint64_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+            tc_mma_f16(tmem + C::T_S + t * 128, dq + off, dk + off, IDESC_S, ks > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
+        };
+        const int n = w.j1 - w.j0;
+        int st = g % C::STAGES;
+        if (!mbar_wait_bounded(&kv_full[st], (g / C::STAGES) & 1, abort_flag, p.errs, kErrAttnWait, 1)) break;
+        tc_fence_after();
+        for (int t = 0; t < w.n_tiles; ++t) issue_s(t, st);
+        for (int j = 0; ok && j < n; ++j) {
+          st = (g + j) % C::STAGES;
+          const int st1 = (g + j + 1) % C::STAGES;
+          if constexpr (!C::QUANT) {
+            if ((w.j0 + j + 1) * 128 > w.visible) {
+              if (!mbar_wait_bounded(&v_zeroed[st], (zeroed_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 7)) {
+                ok = false;
+                break;
+              }
+              zeroed_parity ^= 1u << st;
+            }
+          }
+          bool next_loaded = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || t >= w.n_tiles) break;
+            if (!mbar_wait_bounded(&p_full[t], pn[t] & 1, abort_flag, p.errs, kErrAttnWait, 3 + t)) {
+              ok = false;
+              break;
+            }
+            ++pn[t];
+            if (j == 0 && on[t] > 0 &&
+                !mbar_wait_bounded(&o_free[t], (on[t] - 1) & 1, abort_flag, p.errs, kErrAttnWait, 5 + t)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t dv =
+                smem_desc_sw128(smem_u32(smem + C::KV_OFF + st * C::STAGE_BYTES + C::TILE_BYTES), 16384, 1024);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              tc_mma_f16_ts(tmem + C::T_O + t * C::O_COLS, tmem + C::T_S + t * 128 + ks * 8, dv + ks * (2048 >> 4),
+                            IDESC_O, (j == 0 && ks == 0) ? 0u : 1u);
+            if (j + 1 == n) {
+              tc_commit(&o_done[t]);
+              ++on[t];
+            } else {
+              if (!next_loaded) {
+                if (!mbar_wait_bounded(&kv_full[st1], ((g + j + 1) / C::STAGES) & 1, abort_flag, p.errs, kErrAttnWait,
+                                       1)) {
+                  ok = false;
+                  break;
+                }
+                next_loaded = true;
+                tc_fence_after();
+              }
+              issue_s(t, st1);
+            }
+          }
+          if (!ok) break;
+          tc_commit(&kv_empty[st]);
+        }
+        g += n;
+        tc_commit(&q_empty[qs]);
+        if (!ok || !leave_item(w, p.seqs, shape)) break;
+      }
+    } else if (!C::QUANT && busy && warp == 2) {
+      int g = 0;
+      uint32_t raw_parity = 0;  // bit per stage
+      while (true) {
+        g += w.j1 - w.j0;
+        const int live = w.visible - (w.j1 - 1) * 128;  // only an item's last tile can have a tail
+        if (live < 128) {
+          const int st = (g - 1) % C::STAGES;
+          const bool ok =
+              mbar_wait_bounded(&v_raw[st], (raw_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 8);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          raw_parity ^= 1u << st;
+          uint8_t* vs = smem + C::KV_OFF + st * C::STAGE_BYTES + C::TILE_BYTES;
+          const int dead = 128 - max(live, 0);
+#pragma unroll
+          for (int kb = 0; kb < C::KB; ++kb)
+            for (int i = lane; i < dead * 8; i += 32)
+              *reinterpret_cast<uint4*>(vs + kb * 16384 + (128 - dead) * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_zeroed[st]);
+        }
+        if (!leave_item(w, p.seqs, shape)) break;
+      }
+    }
+  } else if (C::QUANT && warp >= 12) {
+    if constexpr (C::QUANT) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_CONV));
+      const int tid = threadIdx.x - 384;
+      constexpr int PER_ROW = HD / 16;                 // 16-byte pieces of codes per token
+      constexpr int PIECES = 128 * PER_ROW / 128;      // per thread and tile
+      int g = 0;
+      bool ok = busy;
+      while (ok) {
+        const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
+        for (int j = w.j0; j < w.j1; ++j, ++g) {
+          const int st = g % C::STAGES;
+          if (!mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0)) {
+            ok = false;
+            break;
+          }
+          long long cell[PIECES];  // (page, head, offset) of the piece's token, -1: nothing visible there
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) {
+            const int tok = (i * 128 + tid) / PER_ROW;
+            const int t = j * 128 + tok;
+            cell[i] = -1;
+            if (t < w.visible) {
+              const int page = table[t >> page_log2];
+              if (page >= 0 && page < p.seqs.n_pages)
+                cell[i] = (((long long)page * shape.kv_heads + w.it.kvh) << page_log2) + (t & ((1 << page_log2) - 1));
+              else
+                report_error(p.errs, kErrBadIndex, w.it.b);
+            }
+          }
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? p.pool.v : p.pool.k);
+            const float* scales = v ? p.pool.v_scale : p.pool.k_scale;
+            uint8_t* dst = smem + C::KV_OFF + st * C::STAGE_BYTES + v * C::TILE_BYTES;
+            uint4 q[PIECES];
+            float s[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+              const int c = (i * 128 + tid) % PER_ROW;
+              q[i] = make_uint4(0u, 0u, 0u, 0u);
+              s[i] = 0.f;
+              if (cell[i] >= 0) {
+                q[i] = *reinterpret_cast<const uint4*>(src + cell[i] * HD + c * 16);
+                s[i] = scales[cell[i]];
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+              const int id = i * 128 + tid, tok = id / PER_ROW, c = id % PER_ROW;
+              uint4 x[2];
+              expand16<FMT>(q[i], s[i], x);
+              uint8_t* row = dst + (c >> 2) * 16384 + tok * 128;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + h) ^ (tok & 7)) << 4)) = x[h];
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[st]);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok || !leave_item(w, p.seqs, shape)) break;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_HIGH));
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_cols = tmem + lane_off + C::T_S + t * 128;
+    const uint32_t o_cols = tmem + lane_off + C::T_O + t * C::O_COLS;
+    const float scale2 = p.scale * kLog2e;
+    const int tok_in_tile = r / p.group, head = r % p.group;
+    const long long u_begin = w.u;
+    int sn = 0, on = 0;
+    while (busy) {
+      if (t < w.n_tiles) {
+        const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
+        const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
+        const int lim = live ? w.it.seq.len - w.it.seq.qn + tok + 1 : 0;  // tokens that this row sees
+        float m_used = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = w.j0; j < w.j1; ++j) {
+          if (!mbar_wait_bounded(&s_full[t], sn & 1, abort_flag, p.errs, kErrAttnWait, 11 + t)) {
+            ok = false;
+            break;
+          }
+          ++sn;
+          tc_fence_after();
+          uint32_t s[4][32];
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) tmem_ld_32x32b_x32(s_cols + 32 * q4, s[q4]);
+          tc_wait_ld();
+          const int seen = lim - j * 128;
+          if (seen < 128) {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e >= seen) s[e >> 5][e & 31] = __float_as_uint(-INFINITY);
+          }
+          float mx8[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(s[0][e]);
+#pragma unroll
+          for (int e = 8; e < 128; e += 2)
+            mx8[(e >> 1) & 7] = fmax3f(mx8[(e >> 1) & 7], __uint_as_float(s[e >> 5][e & 31]),
+                                       __uint_as_float(s[e >> 5][(e + 1) & 31]));
+          const float mx = fmax3f(fmax3f(mx8[0], mx8[1], mx8[2]), fmax3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+          const float m_row = mx * scale2;
+          if (j == w.j0) {
+            m_used = m_row;
+          } else if (__any_sync(0xffffffffu, m_row > m_used + kRescaleThreshold)) {
+            // taken by the whole warp: tcgen05.ld / st are warp-collective
+            const float m_new = (m_row > m_used + kRescaleThreshold) ? m_row : m_used;
+            const float alpha = m_new == m_used ? 1.f : ex2_approx(m_used - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int cc = 0; cc < HD; cc += 32) {
+              uint32_t ov[32];
+              tmem_ld_32x32b_x32(o_cols + cc, ov);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tmem_st_32x32b_x32(o_cols + cc, ov);
+            }
+            if constexpr (C::ONES) {
+              uint32_t lv[16];
+              tmem_ld_32x32b_x16(o_cols + HD, lv);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) lv[e] = __float_as_uint(__uint_as_float(lv[e]) * alpha);
+              tmem_st_32x32b_x16(o_cols + HD, lv);
+            }
+            m_used = m_new;
+          }
+          const float m_sub = m_used == -INFINITY ? 0.f : m_used;  // nothing seen yet: all probabilities 0
+          float rs8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), scale2, -m_sub));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), scale2, -m_sub));
+            if constexpr (!C::ONES) {
+              rs8[e & 7] += p0;
+              rs8[(e + 1) & 7] += p1;
+            }
+            s[e >> 6][(e >> 1) & 31] = pack_bf16(p0, p1);
+          }
+          if constexpr (!C::ONES)
+            l += ((rs8[0] + rs8[1]) + (rs8[2] + rs8[3])) + ((rs8[4] + rs8[5]) + (rs8[6] + rs8[7]));
+          tmem_st_32x32b_x32(s_cols + 0, s[0]);
+          tmem_st_32x32b_x32(s_cols + 32, s[1]);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        if (!ok) break;
+        if (!mbar_wait_bounded(&o_done[t], on & 1, abort_flag, p.errs, kErrAttnWait, 13 + t)) break;
+        ++on;
+        tc_fence_after();
+        if constexpr (C::ONES) {
+          uint32_t lv[16];
+          tmem_ld_32x32b_x16(o_cols + HD, lv);
+          tc_wait_ld();
+          l = __uint_as_float(lv[0]);
+        }
+        const float inv_l = l == 0.f ? 0.f : 1.0f / l;
+        __nv_bfloat16* dst = p.out + (long long)(w.it.seq.q0 + tok) * p.o_stride_t +
+                             (long long)(w.it.kvh * p.group + head) * p.o_stride_h;
+        // parts go to the workspace as [slot][column / 4][row]: a warp writes 512 contiguous bytes
+        const int slot = 2 * blockIdx.x + (w.u == u_begin ? 0 : 1);
+        const int row = t * 128 + r;
+        float4* part = reinterpret_cast<float4*>(ws.o) + (size_t)slot * (HD / 4) * kItemRows + row;
+#pragma unroll
+        for (int cc = 0; cc < HD; cc += 32) {
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(o_cols + cc, ov);
+          tc_wait_ld();
+          if (cc + 32 >= HD) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[t]);
+          }
+          if (w.whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 x;
+              x.x = pack_bf16(__uint_as_float(ov[e]) * inv_l, __uint_as_float(ov[e + 1]) * inv_l);
+              x.y = pack_bf16(__uint_as_float(ov[e + 2]) * inv_l, __uint_as_float(ov[e + 3]) * inv_l);
+              x.z = pack_bf16(__uint_as_float(ov[e + 4]) * inv_l, __uint_as_float(ov[e + 5]) * inv_l);
+              x.w = pack_bf16(__uint_as_float(ov[e + 6]) * inv_l, __uint_as_float(ov[e + 7]) * inv_l);
+              if (live) *reinterpret_cast<uint4*>(dst + cc + e) = x;
+            }
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              part[(size_t)((cc + e) / 4) * kItemRows] =
+                  make_float4(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1]), __uint_as_float(ov[e + 2]),
+                              __uint_as_float(ov[e + 3]));
+          }
+        }
+        if (!w.whole && live) ws.ml[(size_t)slot * kItemRows + row] = make_float2(m_used, l);
+      }
+      if (!leave_item(w, p.seqs, shape)) break;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// Joins the parts of items that lie in more than one block's range (see paged_join_kernel): a thread per
+// row, 16 columns per block in y.
+template <int HD>
+__global__ void __launch_bounds__(kItemRows)
+    paged_chunk_join_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
+  pdl_wait_and_release();
+  const long long total = ws.total[0];
+  const int blocks = (int)ws.total[1];
+  const int c = blockIdx.x + 1;
+  if (c >= blocks) return;
+  const PagedRecord rec = ws.records[c];
+  const long long before = range_begin(c - 1, total, blocks);
+  if (rec.start == range_begin(c, total, blocks) || before > rec.start) return;
+  const int last = block_of_unit(rec.start + rec.n_units - 1, total, blocks);
+  const int parts = last - c + 2;
+  const int first_slot = 2 * (c - 1) + (before == rec.start ? 0 : 1);
+  const SeqInfo seq = seq_info(p.seqs, rec.b);
+  const int tile_tokens = shape.tile_tokens / 2;
+  const int row = threadIdx.x;
+  const int tok_in_tile = (row & 127) / p.group, head = (row & 127) % p.group;
+  const int tok = rec.rt * shape.tile_tokens + (row >> 7) * tile_tokens + tok_in_tile;
+  if (tok_in_tile >= tile_tokens || tok >= seq.qn) return;
+  float mx = -INFINITY;
+  for (int i = 0; i < parts; ++i) {
+    const int slot = i == 0 ? first_slot : 2 * (c - 1 + i);
+    mx = fmaxf(mx, ws.ml[(size_t)slot * kItemRows + row].x);
+  }
+  float4 acc[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const int slot = i == 0 ? first_slot : 2 * (c - 1 + i);
+    const float2 q = ws.ml[(size_t)slot * kItemRows + row];
+    const float f = q.x == mx ? 1.f : ex2_approx(q.x - mx);
+    l += q.y * f;
+    const float4* src = reinterpret_cast<const float4*>(ws.o) + ((size_t)slot * (HD / 4) + blockIdx.y * 4) * kItemRows + row;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const float4 v = src[d * kItemRows];
+      acc[d].x += v.x * f;
+      acc[d].y += v.y * f;
+      acc[d].z += v.z * f;
+      acc[d].w += v.w * f;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* dst = p.out + (long long)(seq.q0 + tok) * p.o_stride_t +
+                       (long long)(rec.kvh * p.group + head) * p.o_stride_h + blockIdx.y * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint4 x;
+    x.x = pack_bf16(acc[2 * h].x * inv, acc[2 * h].y * inv);
+    x.y = pack_bf16(acc[2 * h].z * inv, acc[2 * h].w * inv);
+    x.z = pack_bf16(acc[2 * h + 1].x * inv, acc[2 * h + 1].y * inv);
+    x.w = pack_bf16(acc[2 * h + 1].z * inv, acc[2 * h + 1].w * inv);
+    *reinterpret_cast<uint4*>(dst + 8 * h) = x;
+  }
+}
+
+template <int FMT, int HD>
+void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
+  using C = ChunkCfg<FMT, HD>;
+  auto* kernel = paged_chunk_kernel<FMT, HD>;
+  static std::atomic<unsigned long long> configured{0};
+  once_per_device(configured, [&] {
+    cudaFuncAttributes attr;
+    B200_CUDA_CHECK(cudaFuncGetAttributes(&attr, kernel));
+    // the register split draws on what the launch gives: with fewer, setmaxnreg would wait for ever
+    B200_CHECK(attr.numRegs * C::THREADS >= C::REGS_NEEDED, "paged attention: built with too few registers");
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+  });
+  const int blocks = num_sms_cached();
+  const PagedWorkspace ws = paged_workspace(alloc(paged_workspace_bytes(blocks, kItemRows, HD)), blocks, kItemRows);
+  const int tile_tokens = 128 / p.group;
+  const PagedShape shape{2 * tile_tokens, 7, p.pool.kv_heads};
+  const CUtensorMap tm_q = make_tmap_bf16_3d(p.q, HD, p.heads, p.seqs.total_q, p.q_stride_h, p.q_stride_t, 64,
+                                             p.group, tile_tokens);
+  CUtensorMap tm_k = tm_q, tm_v = tm_q;  // 8-bit pages are not read by TMA
+  if constexpr (!C::QUANT) {
+    const uint64_t rows = (uint64_t)p.seqs.n_pages * p.pool.kv_heads << p.seqs.page_log2;
+    tm_k = make_tmap_bf16_2d(p.pool.k, HD, rows, HD, 64, 1u << p.seqs.page_log2);
+    tm_v = make_tmap_bf16_2d(p.pool.v, HD, rows, HD, 64, 1u << p.seqs.page_log2);
+  }
+  launch_k(kernel, dim3(blocks), dim3(C::THREADS), C::SMEM_BYTES, s, 1, tm_q, tm_k, tm_v, p, shape, ws);
+  launch_k(paged_chunk_join_kernel<HD>, dim3(blocks - 1, HD / 16), dim3(kItemRows), 0, s, 1, p, shape, ws);
+  B200_CUDA_CHECK(cudaGetLastError());
+  count_launch(2);
+}
+
+}  // namespace
+
+void paged_attention_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
+  const bool hd64 = p.pool.head_dim == 64;
+  switch (p.pool.fmt) {
+    case KV_E4M3: hd64 ? launch_chunk<KV_E4M3, 64>(p, alloc, s) : launch_chunk<KV_E4M3, 128>(p, alloc, s); break;
+    case KV_INT8: hd64 ? launch_chunk<KV_INT8, 64>(p, alloc, s) : launch_chunk<KV_INT8, 128>(p, alloc, s); break;
+    default: hd64 ? launch_chunk<KV_BF16, 64>(p, alloc, s) : launch_chunk<KV_BF16, 128>(p, alloc, s); break;
+  }
+}
+
+}  // namespace b200

@@ -89,11 +89,11 @@ def test_bad_batches(F):
     with pytest.raises(RuntimeError, match="share memory"):
         F.paged_attention(b.q, p, b.table, b.lens, b.starts, 2, out=b.q)
     with pytest.raises(RuntimeError, match="overlap"):
-        F.paged_attention(b.q, p, b.table, b.lens, b.starts, 2, out=torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(3, 4, 64))
+        F.paged_attention(b.q, p, b.table, b.lens, b.starts, 2, out=torch.zeros(999, dtype=torch.bfloat16).as_strided((3, 4, 64), (64, 64, 1)))
     with pytest.raises(RuntimeError, match="scale must be"):
         F.paged_attention(b.q, p, b.table, b.lens, b.starts, 2, scale=float("nan"))
     odd = torch.zeros(3, 4 * 64 + 4, dtype=torch.bfloat16)[:, :256].view(3, 4, 64)
-    with pytest.raises(RuntimeError, match="multiples of 8"):
+    with pytest.raises(RuntimeError, match="positive multiples of 8"):
         F.paged_attention(odd, p, b.table, b.lens, b.starts, 2)
     with pytest.raises(RuntimeError, match="k must be"):
         F.kv_cache_write(p, b.k[:, :1], b.v, b.table, b.lens, b.starts)

@@ -95,6 +95,17 @@ def test_few_tokens_long_cache(F, fmt, q_len):
 
 
 @pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_items_that_span_blocks(F, fmt, hd):
+    """Items of many units, cut by the blocks' ranges, with one tile or two and ends inside a tile: what a
+    stage held before, and what lies behind the sequence in its last page, must not show."""
+    for q, kv in (([200], [1500]), ([1, 17, 200], [3000, 900, 1500]), ([40, 64, 8], [2047, 2049, 1111])):
+        b = Batch(q, kv, 8, 2, hd, fmt, 16, seed=15)
+        want, mag, size = b.attention()
+        _check(_attend(F, b), want, tolerance(want, mag, size, fmt != "bf16"))
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
 def test_rows_before_the_first_token_are_zero(F, fmt):
     """More new tokens than cached ones: the first rows stand before the sequence and see nothing."""
     for q, kv in (([5, 3], [2, 0]), ([200, 150], [60, 0])):
