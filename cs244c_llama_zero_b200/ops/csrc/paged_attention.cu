@@ -4,21 +4,26 @@
 // Row i of a sequence with q_len new of kv_len cached tokens stands at position p = kv_len - q_len + i:
 //   o = sum_{j <= p} softmax_j(scale * q . k_j) v_j      (p < 0: zeros)
 //
-// Few rows (at most 16 per kv head, so one new token in particular): every cached byte is used for a
-// handful of products, and the cache's bandwidth is the bound.  The work is cut into equal runs of 64-token
-// units over all sequences and heads (paged_sched.cuh).  Four warps per block, each on its own 16 tokens of
-// the unit with its own ring of cp.async stages, so that nothing synchronises the warps until a run ends.
-// A page holds a multiple of 16 tokens: the 16 tokens of a warp are one contiguous piece of memory.
+// Few rows (one new token, or a handful): every cached byte is used for a handful of products, and the
+// cache's bandwidth is the bound.  The work is cut into equal runs of 64-token units over all sequences and
+// heads (paged_sched.cuh).  Four warps per block, each on its own 16 tokens of the unit with its own ring of
+// cp.async stages, so that nothing synchronises the warps until a run ends.  A page holds a multiple of 16
+// tokens: the 16 tokens of a warp are one contiguous piece of memory.
 //
 // Products on the warp matrix instructions with the TOKENS along M and the rows along N (S^T = K Q^T,
 // O^T = V^T P^T): with 8 rows along N no part of the instruction is padding for groups of up to 8 heads.
-//   bf16: K by ldmatrix, V^T by ldmatrix.trans.
-//   8-bit: 16-byte shared loads; the codes become bf16 in registers (exactly) by integer operations and one
-//   packed add or multiply, with the order of head_dim inside a product and of O's rows chosen such that a
-//   lane's 16 bytes feed its own fragments.  k_scale multiplies the scores in fp32, v_scale the probabilities
-//   before they are rounded to bf16.
+//   bf16: K by ldmatrix, V^T by ldmatrix.trans, probabilities rounded to bf16.
+//   8-bit: 16-byte shared loads; the codes become fp16 in registers, exactly (e4m3: one conversion per pair;
+//   int8: the code + 128 as the low bits of 1024, less 1152), with the order of head_dim inside a product and
+//   of O's rows chosen such that a lane's 16 bytes feed its own fragments.  A row of q is scaled by a power of
+//   two to a maximum in [1, 2) before it is rounded to fp16, which its 8 bits survive down to 2^-17 of the
+//   maximum.  k_scale multiplies the scores in fp32.  v_scale goes into the exponent: with
+//   x_j = s_j + log2 v_scale_j the weights 2^(x_j - m) that meet the codes have their maximum near 1 whatever
+//   the scales are, so fp16 holds them (the largest at 2^6, errors below 2^-30 of it), and the normaliser
+//   sums 2^(x_j - m) / v_scale_j in fp32.
 // The running maximum is raised only when a score exceeds it by more than 2^8 (one vote per 16 tokens).
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -59,8 +64,16 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -80,27 +93,45 @@ __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&w)[4]) {
 __device__ __forceinline__ void lds64(uint32_t addr, uint32_t& w0, uint32_t& w1) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w0), "=r"(w1) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float lds32f(uint32_t addr) {
   float f;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
   return f;
 }
 
-// Two 8-bit codes, each in both bytes of its 16-bit half of t, as a pair of bf16 (exact).
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if constexpr (!F16) return pack_bf16(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The 8-bit codes (b0, b1) and (b2, b3) of a word as two fp16 pairs, exactly.  int8 codes come with their
+// sign bit flipped (code + 128).
 template <int FMT>
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t t) {
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& p0, uint32_t& p1) {
   if constexpr (FMT == KV_INT8) {
-    // 128 + low 7 bits, minus 128 or (sign bit set) 256: bf16 holds all of these exactly
-    const uint32_t a = (t & 0x007F007Fu) | 0x43004300u, c = (t & 0x00800080u) | 0x43004300u;
-    __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&c));
-    return *reinterpret_cast<uint32_t*>(&d);
+    const uint32_t bias = 0x64806480u;  // 1152
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
+    p0 = *reinterpret_cast<const uint32_t*>(&x);
+    p1 = *reinterpret_cast<const uint32_t*>(&y);
   } else {
-    // exponent and mantissa moved to bf16's places give the value times 2^-120, subnormals included
-    const uint32_t a = ((t << 4) & 0x07F007F0u) | (t & 0x80008000u);
-    const uint32_t unit = 0x7B807B80u;  // 2^120
-    __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&unit));
-    return *reinterpret_cast<uint32_t*>(&d);
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(p0), "=r"(p1)
+        : "r"(w));
   }
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t code_word(uint32_t w) {
+  return FMT == KV_INT8 ? w ^ 0x80808080u : w;
 }
 
 template <int FMT, int HD, int NT>
@@ -112,6 +143,7 @@ struct DecodeCfg {
   static constexpr int SCALES = FMT == KV_BF16 ? 0 : 128;      // 16 fp32 scales of K, 16 of V
   static constexpr int STAGE = 2 * TILE + SCALES;
   static constexpr int STAGES = 3;
+  static constexpr float HEADROOM = FMT == KV_BF16 ? 0.f : 6.f;  // log2 of the largest weight (before lazy raises)
   static constexpr int RING = STAGES * STAGE;                  // per warp
   static constexpr int O_LD = HD + 4;                          // row stride of the merge buffer, in floats
   static constexpr int MERGE = kDecodeWarps * ROWS * O_LD * 4;
@@ -132,11 +164,20 @@ __device__ __forceinline__ uint32_t chunk_offset(int tok, int c) {
     return line * 128 + ((IS_V ? p ^ ((line & 3) << 1) : p) << 4);
   }
 }
+// Pass i of a tile's copy moves 512 bytes, 16 per lane.  Its lanes' offsets are those of pass 0 with these
+// bits flipped, plus 512 i (the row bits that i and the lane contribute are disjoint).
+template <int FMT, int HD, bool IS_V>
+__device__ __forceinline__ constexpr uint32_t pass_flip(int i) {
+  if (FMT == KV_BF16) return (HD == 64 ? (4 * i) & 7 : (2 * i) & 7) << 4;
+  return HD == 128 && IS_V ? ((2 * i) & 3) << 5 : 0;
+}
 
 template <int FMT, int HD, int NT>
 __global__ void __launch_bounds__(kDecodeThreads)
     paged_decode_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
   using C = DecodeCfg<FMT, HD, NT>;
+  constexpr bool QUANT = FMT != KV_BF16;
+  constexpr int KS = HD / 16;  // k-steps of the scores, and 16-column tiles of O
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait_and_release();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -148,7 +189,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
   }
   if ((int)blockIdx.x >= range.blocks) return;
   const long long u_begin = range_begin(blockIdx.x, range.total, range.blocks);
-  const long long u_end = range_begin(blockIdx.x + 1, range.total, range.blocks);
+  int left = (int)(range_begin(blockIdx.x + 1, range.total, range.blocks) - u_begin);  // units to compute
   PagedItem it = item_at(p.seqs, shape, range.b, range.base, u_begin);
   if (threadIdx.x == 0) ws.records[blockIdx.x] = {it.start, it.n_units, it.b, it.kvh, it.rt};
 
@@ -157,79 +198,112 @@ __global__ void __launch_bounds__(kDecodeThreads)
   float2* ml_smem = reinterpret_cast<float2*>(smem + C::ML_OFF);
   const int page_log2 = p.seqs.page_log2, page_mask = (1 << page_log2) - 1;
 
-  // ---- loads: a second walk over the same units, STAGES - 1 ahead
+  // ---- loads: a second walk over the same units, STAGES ahead
   PagedItem li = it;
-  long long lu = u_begin;
-  int slot_in = 0;
-  auto first_page = [&](const PagedItem& x, int t) {  // page of token t of item x, -1 if it has none
-    if (t >= item_visible(x.seq, x.rt, shape.tile_tokens)) return -1;
-    const int page = p.seqs.table[(long long)x.b * p.seqs.table_stride + (t >> page_log2)];
-    if (page >= 0 && page < p.seqs.n_pages) return page;
-    if (lane == 0) report_error(p.errs, kErrBadIndex, x.b);
-    return -1;
+  int l_unit = (int)(u_begin - it.start), l_left = left;
+  int l_visible = item_visible(li.seq, li.rt, shape.tile_tokens);
+  uint32_t slot_in = ring;
+  constexpr int PER_ROW = C::ROW_BYTES / 16;
+  const uint32_t k_off0 = chunk_offset<FMT, HD, false>(lane / PER_ROW, lane % PER_ROW);
+  const uint32_t v_off0 = chunk_offset<FMT, HD, true>(lane / PER_ROW, lane % PER_ROW) + C::TILE;
+  // Page of this warp's tokens of the unit to load (-1: it sees none of them).  Read one unit ahead and
+  // looked at only when the unit is loaded, so that nobody waits for it.
+  auto page_of = [&]() {
+    const int t = l_unit * 64 + 16 * warp;
+    return t < l_visible ? p.seqs.table[(long long)li.b * p.seqs.table_stride + (t >> page_log2)] : -1;
   };
-  int page = first_page(li, (int)(lu - li.start) * 64 + 16 * warp);
+  int page = page_of();
   auto load_unit = [&]() {
-    if (lu < u_end) {
-      const int t0 = (int)(lu - li.start) * 64 + 16 * warp;
-      const int live = page >= 0 ? min(16, item_visible(li.seq, li.rt, shape.tile_tokens) - t0) : 0;
+    if (l_left > 0) {
+      const int t0 = l_unit * 64 + 16 * warp;
+      int live = min(16, l_visible - t0);
+      if (live > 0 && (page < 0 || page >= p.seqs.n_pages)) {
+        if (lane == 0) report_error(p.errs, kErrBadIndex, li.b);
+        live = 0;
+      }
       const long long cell =
           live > 0 ? (((long long)page * shape.kv_heads + li.kvh) << page_log2) + (t0 & page_mask) : 0;
-      const uint32_t dst = ring + slot_in * C::STAGE;
-      constexpr int PER_ROW = C::ROW_BYTES / 16;
+      const uint8_t* k_src = reinterpret_cast<const uint8_t*>(p.pool.k) + cell * C::ROW_BYTES + lane * 16;
+      const uint8_t* v_src = reinterpret_cast<const uint8_t*>(p.pool.v) + cell * C::ROW_BYTES + lane * 16;
+      const uint32_t k_dst = slot_in + k_off0, v_dst = slot_in + v_off0;
+      if (live == 16) {
 #pragma unroll
-      for (int i = 0; i < C::TILE / 512; ++i) {
-        const int id = i * 32 + lane, tok = id / PER_ROW, c = id % PER_ROW;
-        const int bytes = tok < live ? 16 : 0;  // rows behind the last visible token become zeros
-        const size_t off = bytes ? (size_t)cell * C::ROW_BYTES + (size_t)id * 16 : 0;
-        cp_async16(dst + chunk_offset<FMT, HD, false>(tok, c), reinterpret_cast<const uint8_t*>(p.pool.k) + off, bytes);
-        cp_async16(dst + C::TILE + chunk_offset<FMT, HD, true>(tok, c),
-                   reinterpret_cast<const uint8_t*>(p.pool.v) + off, bytes);
+        for (int i = 0; i < C::TILE / 512; ++i) {
+          cp_async16((k_dst ^ pass_flip<FMT, HD, false>(i)) + i * 512, k_src + i * 512, 16);
+          cp_async16((v_dst ^ pass_flip<FMT, HD, true>(i)) + i * 512, v_src + i * 512, 16);
+        }
+      } else {  // rows behind the last visible token become zeros
+#pragma unroll
+        for (int i = 0; i < C::TILE / 512; ++i) {
+          const int bytes = i * (32 / PER_ROW) + lane / PER_ROW < live ? 16 : 0;
+          const int at = bytes ? i * 512 : -lane * 16;  // a copy of no bytes still names a valid address
+          cp_async16((k_dst ^ pass_flip<FMT, HD, false>(i)) + i * 512, k_src + at, bytes);
+          cp_async16((v_dst ^ pass_flip<FMT, HD, true>(i)) + i * 512, v_src + at, bytes);
+        }
       }
-      if constexpr (FMT != KV_BF16) {
+      if constexpr (QUANT) {
         if (lane < 8) {
           const int i = lane & 3;
           const int bytes = max(0, min(16, (live - 4 * i) * 4));
-          const float* src = (lane < 4 ? p.pool.k_scale : p.pool.v_scale) + (bytes ? cell + 4 * i : 0);
-          cp_async16(dst + 2 * C::TILE + lane * 16, src, bytes);
+          const float* src = (lane < 4 ? p.pool.k_scale : p.pool.v_scale) + cell + (bytes ? 4 * i : 0);
+          cp_async16(slot_in + 2 * C::TILE + lane * 16, src, bytes);
         }
       }
-      slot_in = slot_in + 1 == C::STAGES ? 0 : slot_in + 1;
-      if (++lu < u_end) {
-        if (lu == li.start + li.n_units) next_item(li, p.seqs, shape);
-        page = first_page(li, (int)(lu - li.start) * 64 + 16 * warp);
+      slot_in = slot_in + C::STAGE == ring + C::RING ? ring : slot_in + C::STAGE;
+      if (--l_left > 0) {
+        if (++l_unit == li.n_units) {
+          next_item(li, p.seqs, shape);
+          l_unit = 0;
+          l_visible = item_visible(li.seq, li.rt, shape.tile_tokens);
+        }
+        page = page_of();
       }
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < C::STAGES - 1; ++i) load_unit();
+  for (int i = 0; i < C::STAGES; ++i) load_unit();
+
+  // fragment addresses inside a stage (a stage starts on a multiple of 128 bytes: flipping bits 4 to 6 of the
+  // sum flips them in the offset)
+  uint32_t k_frag, v_frag;
+  if constexpr (!QUANT) {
+    k_frag = chunk_offset<FMT, HD, false>(lane & 15, lane >> 4);
+    v_frag = C::TILE + chunk_offset<FMT, HD, true>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+  } else {
+    k_frag = chunk_offset<FMT, HD, false>(n, j);
+    v_frag = C::TILE + (HD == 128 ? chunk_offset<FMT, HD, true>(2 * j, n)
+                                  : chunk_offset<FMT, HD, true>(2 * j, n >> 1) + ((n & 1) << 3));
+  }
 
   const float scale2 = p.scale * kLog2e;
-  int slot_out = 0;
-  long long u = u_begin;
+  uint32_t slot_out = ring;
+  bool first = true;
+  int unit = (int)(u_begin - it.start);
   while (true) {  // one item, or the part of it in this block's range
-    const long long seg_end = min(u_end, it.start + it.n_units);
-    const bool whole = u == it.start && seg_end == it.start + it.n_units;
-    const bool first = u == u_begin;
+    const int seg = min(left, it.n_units - unit);
+    const bool whole = seg == it.n_units;
     const int tok0 = it.rt * shape.tile_tokens;
     const int rows = min(shape.tile_tokens, it.seq.qn - tok0) * p.group;
     const int base_pos = it.seq.len - it.seq.qn + tok0;  // position of the item's first row
+    const int visible = item_visible(it.seq, it.rt, shape.tile_tokens);
     // Q^T fragments; rows that do not exist are zeros
-    uint32_t qf[NT][HD / 16][2];
+    uint32_t qf[NT][KS][2];
+    float q_unit[NT][2];  // 8-bit: what the scores of rows 2 j and 2 j + 1 are multiplied by
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = 8 * t + n;
       const bool ok = r < rows;
       const __nv_bfloat16* src = p.q + (long long)(it.seq.q0 + tok0 + r / p.group) * p.q_stride_t +
                                  (long long)(it.kvh * p.group + r % p.group) * p.q_stride_h;
-      if constexpr (FMT == KV_BF16) {
+      if constexpr (!QUANT) {
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
+        for (int ks = 0; ks < KS; ++ks) {
           qf[t][ks][0] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j) : 0u;
           qf[t][ks][1] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j + 8) : 0u;
         }
-      } else {  // product 4 g + s takes columns 64 g + 16 j + 4 s + {0, 2} and {1, 3}
+      } else {  // product 4 g + x takes columns 64 g + 16 j + 4 x + {0, 1} and {2, 3}
+        uint32_t top = 0u;
 #pragma unroll
         for (int g = 0; g < HD / 64; ++g) {
           uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
@@ -239,28 +313,31 @@ __global__ void __launch_bounds__(kDecodeThreads)
           }
           const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            qf[t][4 * g + s][0] = __byte_perm(x[2 * s], x[2 * s + 1], 0x5410);
-            qf[t][4 * g + s][1] = __byte_perm(x[2 * s], x[2 * s + 1], 0x7632);
+          for (int k = 0; k < 4; ++k) {
+            qf[t][4 * g + k][0] = x[2 * k];
+            qf[t][4 * g + k][1] = x[2 * k + 1];
+            top = __vmaxu2(top, __vmaxu2(x[2 * k] & 0x7FFF7FFFu, x[2 * k + 1] & 0x7FFF7FFFu));
           }
         }
+        uint32_t m = max(top & 0xFFFFu, top >> 16);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = min(max((int)(m >> 7), 2), 252);  // biased exponent of the row's maximum
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            qf[t][ks][h] = pack_pair<true>(bf16lo(qf[t][ks][h]) * down, bf16hi(qf[t][ks][h]) * down);
+        q_unit[t][0] = scale2 * __shfl_sync(0xffffffffu, up, 8 * j);
+        q_unit[t][1] = scale2 * __shfl_sync(0xffffffffu, up, 8 * j + 4);
       }
     }
-    // visible tokens of the rows this lane holds scores of, and the fewest of any row
-    int lim[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * t + 2 * j + e;
-        lim[t][e] = r < rows ? base_pos + r / p.group + 1 : 0x7FFFFFFF;
-      }
-    const int all_see = base_pos + 1;
-    const int visible = item_visible(it.seq, it.rt, shape.tile_tokens);
+    const int all_see = base_pos + 1;  // fewest visible tokens of any row
 
-    float o[HD / 16][NT][4];
+    float o[KS][NT][4];
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i)
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -269,66 +346,76 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
     for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
 
-    for (; u < seg_end; ++u) {
-      load_unit();
+    for (int c = 0; c < seg; ++c, ++unit) {
       cp_async_wait<C::STAGES - 1>();
       __syncwarp();
-      const uint32_t ks_tile = ring + slot_out * C::STAGE, vs_tile = ks_tile + C::TILE;
-      const int t0 = (int)(u - it.start) * 64 + 16 * warp;
+      const int t0 = unit * 64 + 16 * warp;
       if (t0 < visible) {
+        const uint32_t ka = slot_out + k_frag, va = slot_out + v_frag;
         float s[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        if constexpr (FMT == KV_BF16) {
-          const int tok = lane & 15;
+        if constexpr (!QUANT) {
 #pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
+          for (int ks = 0; ks < KS; ++ks) {
             uint32_t a[4];
-            ldsm_x4(ks_tile + chunk_offset<FMT, HD, false>(tok, 2 * ks + (lane >> 4)), a);
+            ldsm_x4((ka ^ (((2 * ks) & 7) << 4)) + (ks >> 2) * 128, a);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_bf16(s[t], a, qf[t][ks][0], qf[t][ks][1]);
+            for (int t = 0; t < NT; ++t) mma_16816<false>(s[t], a, qf[t][ks][0], qf[t][ks][1]);
           }
         } else {
 #pragma unroll
           for (int g = 0; g < HD / 64; ++g) {
             uint32_t lo[4], hi[4];
-            lds128(ks_tile + chunk_offset<FMT, HD, false>(n, 4 * g + j), lo);
-            lds128(ks_tile + chunk_offset<FMT, HD, false>(n + 8, 4 * g + j), hi);
+            lds128(ka ^ (g << 6), lo);
+            lds128((ka ^ (g << 6)) + 8 * HD, hi);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const uint32_t a[4] = {codes_to_bf16<FMT>(__byte_perm(lo[x], 0, 0x2200)),
-                                     codes_to_bf16<FMT>(__byte_perm(hi[x], 0, 0x2200)),
-                                     codes_to_bf16<FMT>(__byte_perm(lo[x], 0, 0x3311)),
-                                     codes_to_bf16<FMT>(__byte_perm(hi[x], 0, 0x3311))};
+              uint32_t a[4];
+              codes_to_f16<FMT>(code_word<FMT>(lo[x]), a[0], a[2]);
+              codes_to_f16<FMT>(code_word<FMT>(hi[x]), a[1], a[3]);
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma_bf16(s[t], a, qf[t][4 * g + x][0], qf[t][4 * g + x][1]);
+              for (int t = 0; t < NT; ++t) mma_16816<true>(s[t], a, qf[t][4 * g + x][0], qf[t][4 * g + x][1]);
             }
           }
         }
-        // scores in log2 units
-        float kf0 = scale2, kf1 = scale2, vf0 = 1.f, vf1 = 1.f;
-        if constexpr (FMT != KV_BF16) {
-          kf0 *= lds32f(ks_tile + 2 * C::TILE + n * 4);
-          kf1 *= lds32f(ks_tile + 2 * C::TILE + n * 4 + 32);
-          vf0 = lds32f(ks_tile + 2 * C::TILE + 64 + n * 4);
-          vf1 = lds32f(ks_tile + 2 * C::TILE + 64 + n * 4 + 32);
+        // scores in log2 units; 8-bit: plus log2 of v_scale, with w = 1 / v_scale for the normaliser
+        float w0 = 1.f, w1 = 1.f;
+        if constexpr (QUANT) {
+          const uint32_t sa = slot_out + 2 * C::TILE + n * 4;
+          const float k0 = lds32f(sa), k1 = lds32f(sa + 32), v0 = lds32f(sa + 64), v1 = lds32f(sa + 96);
+          // a scale of 0 (all codes 0) counts as 2^-100; a NaN stays one
+          const float x0 = lg2_approx(fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
+          const float x1 = lg2_approx(fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
+          w0 = ex2_approx(-x0);
+          w1 = ex2_approx(-x1);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            s[t][0] = fmaf(s[t][0], k0 * q_unit[t][0], x0);
+            s[t][1] = fmaf(s[t][1], k0 * q_unit[t][1], x0);
+            s[t][2] = fmaf(s[t][2], k1 * q_unit[t][0], x1);
+            s[t][3] = fmaf(s[t][3], k1 * q_unit[t][1], x1);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] *= scale2;
+        }
+        if (t0 + 16 > all_see) {  // a row that does not exist is masked like the last one
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int lim = min(base_pos + (8 * t + 2 * j + e) / p.group + 1, visible);
+              if (t0 + n >= lim) s[t][e] = -INFINITY;
+              if (t0 + n + 8 >= lim) s[t][2 + e] = -INFINITY;
+            }
         }
         bool raise = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s[t][0] *= kf0;
-          s[t][1] *= kf0;
-          s[t][2] *= kf1;
-          s[t][3] *= kf1;
-          if (t0 + 16 > all_see) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (t0 + n >= min(lim[t][e], visible)) s[t][e] = -INFINITY;
-              if (t0 + n + 8 >= min(lim[t][e], visible)) s[t][2 + e] = -INFINITY;
-            }
-          }
+        for (int t = 0; t < NT; ++t)
           raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise || fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
-        }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -343,7 +430,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
               m[t][e] = m_new;
               l[t][e] *= alpha;
 #pragma unroll
-              for (int i = 0; i < HD / 16; ++i) {
+              for (int i = 0; i < KS; ++i) {
                 o[i][t][e] *= alpha;
                 o[i][t][2 + e] *= alpha;
               }
@@ -352,52 +439,56 @@ __global__ void __launch_bounds__(kDecodeThreads)
         uint32_t pf[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+          // nothing seen yet: all weights 0
+          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0] - C::HEADROOM;
+          const float m1 = m[t][1] == -INFINITY ? 0.f : m[t][1] - C::HEADROOM;
           const float p0 = ex2_approx(s[t][0] - m0), p1 = ex2_approx(s[t][1] - m1);
           const float p2 = ex2_approx(s[t][2] - m0), p3 = ex2_approx(s[t][3] - m1);
-          l[t][0] += p0 + p2;
-          l[t][1] += p1 + p3;
-          // rounded to bf16 for the product with V: half a step of 2^-8 relative for each probability
-          pf[t][0] = transpose_8x8(pack_bf16(p0 * vf0, p1 * vf0));
-          pf[t][1] = transpose_8x8(pack_bf16(p2 * vf1, p3 * vf1));
+          l[t][0] += QUANT ? fmaf(p0, w0, p2 * w1) : p0 + p2;
+          l[t][1] += QUANT ? fmaf(p1, w0, p3 * w1) : p1 + p3;
+          // rounded for the product with V (bf16: half a step of 2^-8 relative for each probability)
+          pf[t][0] = transpose_8x8(pack_pair<QUANT>(p0, p1));
+          pf[t][1] = transpose_8x8(pack_pair<QUANT>(p2, p3));
         }
-        if constexpr (FMT == KV_BF16) {
-          const int tok = (lane & 7) + ((lane >> 4) << 3);
+        if constexpr (!QUANT) {
 #pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
+          for (int i = 0; i < KS; ++i) {
             uint32_t a[4];
-            ldsm_x4_t(vs_tile + chunk_offset<FMT, HD, true>(tok, 2 * i + ((lane >> 3) & 1)), a);
+            ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_bf16(o[i][t], a, pf[t][0], pf[t][1]);
+            for (int t = 0; t < NT; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
           }
         } else {
-          // tile i: O's rows n and n + 8 are columns n * HD / 8 + 2 i and + 1 of V
-          constexpr int W = HD / 32;  // words per lane and token
+          // tile i: O's rows n and n + 8 are columns n * HD / 8 + 2 i and + 1 of V; words of tokens
+          // 2 j, 2 j + 1, 2 j + 8, 2 j + 9
+          constexpr int W = HD / 32;
           uint32_t w[4][W];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int tok = 2 * j + (x & 1) + ((x >> 1) << 3);
-            if constexpr (HD == 128) {
-              lds128(vs_tile + chunk_offset<FMT, HD, true>(tok, n), w[x]);
-            } else {
-              lds64(vs_tile + chunk_offset<FMT, HD, true>(tok, n >> 1) + ((n & 1) << 3), w[x][0], w[x][1]);
-            }
+          if constexpr (HD == 128) {
+            lds128(va, w[0]);
+            lds128(va + 128, w[1]);
+            lds128(va + 1024, w[2]);
+            lds128(va + 1152, w[3]);
+          } else {
+            lds64(va, w[0][0], w[0][1]);
+            lds64(va ^ 64, w[1][0], w[1][1]);
+            lds64(va + 512, w[2][0], w[2][1]);
+            lds64((va ^ 64) + 512, w[3][0], w[3][1]);
           }
 #pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
+          for (int i = 0; i < KS; ++i) {
             const int k = i >> 1;
-            const uint32_t s0 = (i & 1) ? 0x6622u : 0x4400u, s1 = (i & 1) ? 0x7733u : 0x5511u;
-            const uint32_t a[4] = {codes_to_bf16<FMT>(__byte_perm(w[0][k], w[1][k], s0)),
-                                   codes_to_bf16<FMT>(__byte_perm(w[0][k], w[1][k], s1)),
-                                   codes_to_bf16<FMT>(__byte_perm(w[2][k], w[3][k], s0)),
-                                   codes_to_bf16<FMT>(__byte_perm(w[2][k], w[3][k], s1))};
+            const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+            uint32_t a[4];
+            codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[0][k], w[1][k], sel)), a[0], a[1]);
+            codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[2][k], w[3][k], sel)), a[2], a[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_bf16(o[i][t], a, pf[t][0], pf[t][1]);
+            for (int t = 0; t < NT; ++t) mma_16816<true>(o[i][t], a, pf[t][0], pf[t][1]);
           }
         }
       }
       __syncwarp();  // every lane has read the stage before it is loaded again
-      slot_out = slot_out + 1 == C::STAGES ? 0 : slot_out + 1;
+      load_unit();
+      slot_out = slot_out + C::STAGE == ring + C::RING ? ring : slot_out + C::STAGE;
     }
 
     // ---- join the four warps
@@ -415,15 +506,16 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * t + 2 * j + e;
+        if (r >= rows) continue;
         float mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kDecodeWarps; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
         const float f = m[t][e] == mx ? 1.f : ex2_approx(m[t][e] - mx);
         float* dst = merge + (warp * C::ROWS + r) * C::O_LD;
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const int d0 = FMT == KV_BF16 ? 16 * i + n : n * (HD / 8) + 2 * i;
-          const int d1 = FMT == KV_BF16 ? d0 + 8 : d0 + 1;
+        for (int i = 0; i < KS; ++i) {
+          const int d0 = QUANT ? n * (HD / 8) + 2 * i : 16 * i + n;
+          const int d1 = QUANT ? d0 + 1 : d0 + 8;
           dst[d0] = o[i][t][e] * f;
           dst[d1] = o[i][t][2 + e] * f;
         }
@@ -456,8 +548,11 @@ __global__ void __launch_bounds__(kDecodeThreads)
         if (d == 0) ws.ml[(size_t)slot * C::ROWS + r] = make_float2(mx, sum);
       }
     }
-    if (u == u_end) break;
+    left -= seg;
+    if (left == 0) break;
+    first = false;
     next_item(it, p.seqs, shape);
+    unit = 0;
     __syncthreads();  // the merge buffers are free
   }
   cp_async_wait<0>();
@@ -590,6 +685,10 @@ void launch_rows(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t
     launch_decode<FMT, HD, 1>(p, alloc, s);
   else if (rows <= 16)
     launch_decode<FMT, HD, 2>(p, alloc, s);
+  else if (rows <= 32)
+    launch_decode<FMT, HD, 4>(p, alloc, s);
+  else if (HD == 64 && rows <= 64)
+    launch_decode<FMT, 64, 8>(p, alloc, s);
   else
     paged_attention_chunk(p, alloc, s);
 }

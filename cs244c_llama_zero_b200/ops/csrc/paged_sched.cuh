@@ -169,7 +169,7 @@ __device__ inline PagedRange find_range(const PagedSeqs& s, const PagedShape& sh
     long long at = before + incl - mine;
     if (u >= at && u < at + mine) {
       for (int b = b0; b < b1; ++b) {
-        const long long n = head_units(seq_info(s, b), sh) * sh.kv_heads;
+        const long long n = b1 - b0 == 1 ? mine : head_units(seq_info(s, b), sh) * sh.kv_heads;
         if (u < at + n) {
           found[0] = b;
           found[1] = at;
