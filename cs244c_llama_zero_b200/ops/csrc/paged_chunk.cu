@@ -49,10 +49,12 @@ struct ChunkCfg {
   static constexpr int TILE_BYTES = 128 * HD * 2;
   static constexpr int STAGES = (HD == 64) ? 3 : 2;
   static constexpr int Q_BUFS = (HD == 64) ? 2 : 1;
-  static constexpr int REGS_LOW = QUANT ? 48 : 88;
-  static constexpr int REGS_CONV = QUANT ? 80 : 0;
-  static constexpr int REGS_HIGH = QUANT ? 192 : 208;
-  static constexpr int REGS_NEEDED = 128 * REGS_LOW + 256 * REGS_HIGH + 128 * REGS_CONV;
+  // bf16: a softmax thread keeps its row's 128 scores in registers, for which the first warpgroup hands over
+  // some of its own.  8-bit: the expanding warpgroup leaves 128 registers per thread, and the scores are read
+  // from tensor memory twice, 32 at a time (holding them spilled, and a unit took 7 us instead of SOON).
+  static constexpr int REGS_LOW = 88;
+  static constexpr int REGS_HIGH = 208;
+  static constexpr int REGS_NEEDED = QUANT ? 0 : 128 * REGS_LOW + 256 * REGS_HIGH;
   static_assert(REGS_NEEDED <= THREADS * LAUNCH_REGS, "register split over budget");
   // hd 64: row sums from the tensor cores, by a block of ones behind V (see the training forward kernel)
   static constexpr bool ONES = (HD == 64);
@@ -62,36 +64,47 @@ struct ChunkCfg {
   static constexpr int KV_OFF = Q_BUFS * 2 * TILE_BYTES;
   static constexpr int BAR_OFF = KV_OFF + STAGES * STAGE_BYTES;
   static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
-  static_assert(SMEM_BYTES + 512 <= 232448, "shared memory exceeds 227 KB");
+  static_assert(SMEM_BYTES + 2048 <= 232448, "shared memory exceeds 227 KB");
   static constexpr int TMEM_COLS = 512;
   static constexpr int T_S = 0;
   static constexpr int T_O = 256;
   static_assert(T_O + 2 * O_COLS <= TMEM_COLS, "tensor memory");
 };
 
-// One block's walk over its items, the same in every role.
+// A role's walk over its block's items.  Kept in shared memory, one for each warp and advanced by its lane 0:
+// in registers it would spill inside the hot loops of the softmax.
 struct ChunkWalk {
   PagedItem it;
-  long long u, u_end;
   int j0, j1;      // units of the item in this block's range
+  int left;        // units from j0 to the end of the range
   int n_tiles;     // 1: the item has rows in tile A only
   int visible;     // cached tokens that its last row sees
-  bool whole;
 };
-__device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh) {
-  const long long end = w.it.start + w.it.n_units;
-  w.j0 = (int)(w.u - w.it.start);
-  w.j1 = (int)((w.u_end < end ? w.u_end : end) - w.it.start);
-  w.whole = w.j0 == 0 && w.j1 == w.it.n_units;
+__device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh, int j0, int left) {
+  w.j0 = j0;
+  w.left = left;
+  w.j1 = min(w.it.n_units, j0 + left);
   w.n_tiles = w.it.seq.qn - w.it.rt * sh.tile_tokens > sh.tile_tokens / 2 ? 2 : 1;
   w.visible = item_visible(w.it.seq, w.it.rt, sh.tile_tokens);
 }
-__device__ __forceinline__ bool leave_item(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh) {
-  w.u += w.j1 - w.j0;
-  if (w.u == w.u_end) return false;
-  next_item(w.it, s, sh);
-  enter_item(w, sh);
+// By one thread.  False at the end of the range.
+__device__ __forceinline__ bool next_part(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh) {
+  const int left = w.left - (w.j1 - w.j0);
+  if (left == 0) return false;
+  PagedItem it = w.it;
+  next_item(it, s, sh);
+  w.it = it;
+  enter_item(w, sh, 0, left);
   return true;
+}
+// By a whole warp.
+__device__ __forceinline__ bool next_part_warp(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh, int lane) {
+  __syncwarp();
+  bool more = false;
+  if (lane == 0) more = next_part(w, s, sh);
+  more = __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+  __syncwarp();
+  return more;
 }
 
 // 16 codes times their row's scale as 16 bf16.
@@ -121,6 +134,27 @@ __device__ __forceinline__ void expand16(const uint4& q, float scale, uint4 (&ou
   }
   out[0] = make_uint4(r[0], r[1], r[2], r[3]);
   out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// Waits for the tensor-memory loads in flight, and ties the registers of one of them to the wait: another
+// load is issued right behind it, and nothing else keeps the uses of these from moving before the wait.
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// Scores from column `seen` on become -inf.
+__device__ __forceinline__ void mask32(uint32_t (&s)[32], int seen) {
+  if (seen < 32) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (e >= seen) s[e] = 0xFF800000u;
+  }
 }
 
 template <int FMT, int HD>
@@ -190,19 +224,21 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     ws.total[1] = range.blocks;
   }
   const bool busy = (int)blockIdx.x < range.blocks;
-  ChunkWalk w;
-  if (busy) {
-    w.u = range_begin(blockIdx.x, range.total, range.blocks);
-    w.u_end = range_begin(blockIdx.x + 1, range.total, range.blocks);
-    w.it = item_at(p.seqs, shape, range.b, range.base, w.u);
-    enter_item(w, shape);
-    if (threadIdx.x == 0) ws.records[blockIdx.x] = {w.it.start, w.it.n_units, w.it.b, w.it.kvh, w.it.rt};
+  __shared__ ChunkWalk walks[C::THREADS / 32];
+  ChunkWalk& w = walks[warp];
+  if (busy && lane == 0) {
+    const long long u = range_begin(blockIdx.x, range.total, range.blocks);
+    const PagedItem it = item_at(p.seqs, shape, range.b, range.base, u);
+    w.it = it;
+    enter_item(w, shape, (int)(u - it.start), (int)(range_begin(blockIdx.x + 1, range.total, range.blocks) - u));
+    if (warp == 0) ws.records[blockIdx.x] = {it.start, it.n_units, it.b, it.kvh, it.rt};
   }
+  __syncwarp();
   const int tile_tokens = shape.tile_tokens / 2;  // of one tile
   const int page_log2 = p.seqs.page_log2;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_LOW));
+    if constexpr (!C::QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_LOW));
     if (busy && warp == 0 && lane == 0) {
       tma_prefetch_desc(&tm_q);
       int g = 0;
@@ -221,8 +257,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                         w.it.seq.q0 + w.it.rt * shape.tile_tokens + t * tile_tokens);
         if constexpr (!C::QUANT) {
           const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
-          const int page_size = 1 << page_log2;
-          for (int j = w.j0; j < w.j1; ++j, ++g) {
+          const int page_size = 1 << page_log2, kvh = w.it.kvh, visible = w.visible, j1 = w.j1;
+          for (int j = w.j0; j < j1; ++j, ++g) {
             const int st = g % C::STAGES;
             if (!mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0)) {
               ok = false;
@@ -230,9 +266,9 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             }
             uint8_t* ks = smem + C::KV_OFF + st * C::STAGE_BYTES;
             uint8_t* vs = ks + C::TILE_BYTES;
-            const int n_pages = min(128 >> page_log2, max(0, (w.visible - j * 128 + page_size - 1) >> page_log2));
+            const int n_pages = min(128 >> page_log2, max(0, (visible - j * 128 + page_size - 1) >> page_log2));
             // a tile that the sequence ends in gets V on a barrier of its own: warp 2 zeroes its tail first
-            const bool tail = (j + 1) * 128 > w.visible;
+            const bool tail = (j + 1) * 128 > visible;
             uint64_t* v_bar = tail ? &v_raw[st] : &kv_full[st];
             const int bytes = n_pages * page_size * HD * 2;
             mbar_expect_tx(&kv_full[st], tail ? bytes : 2 * bytes);
@@ -243,7 +279,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                 report_error(p.errs, kErrBadIndex, w.it.b);
                 page = p.seqs.n_pages;  // behind the tensor: the copy fills zeros
               }
-              const int row = (int)(min((long long)page * shape.kv_heads + w.it.kvh,
+              const int row = (int)(min((long long)page * shape.kv_heads + kvh,
                                         (long long)p.seqs.n_pages * shape.kv_heads)
                                     << page_log2);
               const int at = i * page_size * 128;
@@ -255,7 +291,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             }
           }
         }
-        if (!ok || !leave_item(w, p.seqs, shape)) break;
+        if (!ok || !next_part(w, p.seqs, shape)) break;
       }
     } else if (busy && warp == 1 && lane == 0) {
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false);
@@ -278,16 +314,16 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           }
           tc_commit(&s_full[t]);
         };
-        const int n = w.j1 - w.j0;
+        const int j0 = w.j0, n = w.j1 - j0, n_tiles = w.n_tiles, visible = w.visible;
         int st = g % C::STAGES;
         if (!mbar_wait_bounded(&kv_full[st], (g / C::STAGES) & 1, abort_flag, p.errs, kErrAttnWait, 1)) break;
         tc_fence_after();
-        for (int t = 0; t < w.n_tiles; ++t) issue_s(t, st);
+        for (int t = 0; t < n_tiles; ++t) issue_s(t, st);
         for (int j = 0; ok && j < n; ++j) {
           st = (g + j) % C::STAGES;
           const int st1 = (g + j + 1) % C::STAGES;
           if constexpr (!C::QUANT) {
-            if ((w.j0 + j + 1) * 128 > w.visible) {
+            if ((j0 + j + 1) * 128 > visible) {
               if (!mbar_wait_bounded(&v_zeroed[st], (zeroed_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 7)) {
                 ok = false;
                 break;
@@ -298,7 +334,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           bool next_loaded = false;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (!ok || t >= w.n_tiles) break;
+            if (!ok || t >= n_tiles) break;
             if (!mbar_wait_bounded(&p_full[t], pn[t] & 1, abort_flag, p.errs, kErrAttnWait, 3 + t)) {
               ok = false;
               break;
@@ -337,7 +373,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         }
         g += n;
         tc_commit(&q_empty[qs]);
-        if (!ok || !leave_item(w, p.seqs, shape)) break;
+        if (!ok || !next_part(w, p.seqs, shape)) break;
       }
     } else if (!C::QUANT && busy && warp == 2) {
       int g = 0;
@@ -361,77 +397,96 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_zeroed[st]);
         }
-        if (!leave_item(w, p.seqs, shape)) break;
+        if (!next_part_warp(w, p.seqs, shape, lane)) break;
       }
     }
   } else if (C::QUANT && warp >= 12) {
     if constexpr (C::QUANT) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_CONV));
+      // K and V of a tile in turn: the next one's codes are in flight while one is expanded, page ids are read
+      // a tile ahead.
       const int tid = threadIdx.x - 384;
-      constexpr int PER_ROW = HD / 16;                 // 16-byte pieces of codes per token
-      constexpr int PIECES = 128 * PER_ROW / 128;      // per thread and tile
-      int g = 0;
-      bool ok = busy;
-      while (ok) {
-        const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
-        for (int j = w.j0; j < w.j1; ++j, ++g) {
-          const int st = g % C::STAGES;
-          if (!mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0)) {
-            ok = false;
-            break;
+      constexpr int PER_ROW = HD / 16;        // pieces per token
+      constexpr int PIECES = PER_ROW;         // per thread and tile: tokens tid / PER_ROW + i * 128 / PER_ROW
+      const int piece = tid % PER_ROW, tok0 = tid / PER_ROW;
+      int cell[PIECES], next_page[PIECES];    // cell: (page, head, offset) index, -1 if nothing is visible there
+      uint4 q[2][PIECES];
+      float sc[2][PIECES];
+      int j = busy ? w.j0 : 0;
+      auto read_pages = [&]() {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int t = j * 128 + tok0 + i * (128 / PER_ROW);
+          next_page[i] = t < w.visible ? p.seqs.table[(long long)w.it.b * p.seqs.table_stride + (t >> page_log2)] : -1;
+        }
+      };
+      auto resolve = [&]() {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int t = j * 128 + tok0 + i * (128 / PER_ROW);
+          const int page = next_page[i];
+          cell[i] = -1;
+          if (page >= 0 && page < p.seqs.n_pages)
+            cell[i] = ((page * shape.kv_heads + w.it.kvh) << page_log2) + (t & ((1 << page_log2) - 1));
+          else if (t < w.visible)
+            report_error(p.errs, kErrBadIndex, w.it.b);
+        }
+      };
+      auto load_codes = [&](int v) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? p.pool.v : p.pool.k) + piece * 16;
+        const float* scales = v ? p.pool.v_scale : p.pool.k_scale;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int c = cell[i];
+          q[v][i] = make_uint4(0u, 0u, 0u, 0u);
+          sc[v][i] = 0.f;
+          if (c >= 0) {
+            q[v][i] = *reinterpret_cast<const uint4*>(src + (long long)c * HD);
+            sc[v][i] = scales[c];
           }
-          long long cell[PIECES];  // (page, head, offset) of the piece's token, -1: nothing visible there
+        }
+      };
+      if (busy) {
+        read_pages();
+        resolve();
+        load_codes(0);
+      }
+      for (int g = 0; busy; ++g) {
+        const int st = g % C::STAGES;
+        bool more = true;
+        if (++j == w.j1) {
+          more = next_part_warp(w, p.seqs, shape, lane);
+          j = 0;
+        }
+        if (more) read_pages();
+        bool ok = true;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          if (v == 0) {
+            load_codes(1);
+            ok = mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0);
+          } else if (more) {
+            resolve();
+            load_codes(0);
+          }
+          uint8_t* dst = smem + C::KV_OFF + st * C::STAGE_BYTES + v * C::TILE_BYTES + (piece >> 2) * 16384;
 #pragma unroll
           for (int i = 0; i < PIECES; ++i) {
-            const int tok = (i * 128 + tid) / PER_ROW;
-            const int t = j * 128 + tok;
-            cell[i] = -1;
-            if (t < w.visible) {
-              const int page = table[t >> page_log2];
-              if (page >= 0 && page < p.seqs.n_pages)
-                cell[i] = (((long long)page * shape.kv_heads + w.it.kvh) << page_log2) + (t & ((1 << page_log2) - 1));
-              else
-                report_error(p.errs, kErrBadIndex, w.it.b);
-            }
+            const int tok = tok0 + i * (128 / PER_ROW);
+            uint4 x[2];
+            expand16<FMT>(q[v][i], sc[v][i], x);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (ok) *reinterpret_cast<uint4*>(dst + tok * 128 + ((((piece & 3) * 2 + h) ^ (tok & 7)) << 4)) = x[h];
           }
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? p.pool.v : p.pool.k);
-            const float* scales = v ? p.pool.v_scale : p.pool.k_scale;
-            uint8_t* dst = smem + C::KV_OFF + st * C::STAGE_BYTES + v * C::TILE_BYTES;
-            uint4 q[PIECES];
-            float s[PIECES];
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-              const int c = (i * 128 + tid) % PER_ROW;
-              q[i] = make_uint4(0u, 0u, 0u, 0u);
-              s[i] = 0.f;
-              if (cell[i] >= 0) {
-                q[i] = *reinterpret_cast<const uint4*>(src + cell[i] * HD + c * 16);
-                s[i] = scales[cell[i]];
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-              const int id = i * 128 + tid, tok = id / PER_ROW, c = id % PER_ROW;
-              uint4 x[2];
-              expand16<FMT>(q[i], s[i], x);
-              uint8_t* row = dst + (c >> 2) * 16384 + tok * 128;
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + h) ^ (tok & 7)) << 4)) = x[h];
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_full[st]);
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok || !leave_item(w, p.seqs, shape)) break;
+        fence_proxy_async_smem();
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) mbar_arrive(&kv_full[st]);
+        if (!more) break;
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_HIGH));
+    if constexpr (!C::QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_HIGH));
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
@@ -440,42 +495,57 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     const uint32_t o_cols = tmem + lane_off + C::T_O + t * C::O_COLS;
     const float scale2 = p.scale * kLog2e;
     const int tok_in_tile = r / p.group, head = r % p.group;
-    const long long u_begin = w.u;
     int sn = 0, on = 0;
-    while (busy) {
+    for (int part_no = 0; busy; ++part_no) {
       if (t < w.n_tiles) {
         const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
         const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
         const int lim = live ? w.it.seq.len - w.it.seq.qn + tok + 1 : 0;  // tokens that this row sees
         float m_used = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = w.j0; j < w.j1; ++j) {
+        const int j0 = w.j0, j1 = w.j1;
+        for (int j = j0; j < j1; ++j) {
           if (!mbar_wait_bounded(&s_full[t], sn & 1, abort_flag, p.errs, kErrAttnWait, 11 + t)) {
             ok = false;
             break;
           }
           ++sn;
           tc_fence_after();
-          uint32_t s[4][32];
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) tmem_ld_32x32b_x32(s_cols + 32 * q4, s[q4]);
-          tc_wait_ld();
           const int seen = lim - j * 128;
-          if (seen < 128) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e >= seen) s[e >> 5][e & 31] = __float_as_uint(-INFINITY);
-          }
+          uint32_t s[C::QUANT ? 2 : 4][32];  // 8-bit: two buffers of 32 scores, else the row's 128
           float mx8[8];
+          if constexpr (C::QUANT) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(s[0][e]);
+            for (int e = 0; e < 8; ++e) mx8[e] = -INFINITY;
+            tmem_ld_32x32b_x32(s_cols, s[0]);
 #pragma unroll
-          for (int e = 8; e < 128; e += 2)
-            mx8[(e >> 1) & 7] = fmax3f(mx8[(e >> 1) & 7], __uint_as_float(s[e >> 5][e & 31]),
-                                       __uint_as_float(s[e >> 5][(e + 1) & 31]));
+            for (int q4 = 0; q4 < 4; ++q4) {
+              tmem_arrived(s[q4 & 1]);
+              if (q4 < 3) tmem_ld_32x32b_x32(s_cols + 32 * (q4 + 1), s[(q4 + 1) & 1]);
+              mask32(s[q4 & 1], seen - 32 * q4);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2)
+                mx8[(e >> 1) & 7] = fmax3f(mx8[(e >> 1) & 7], __uint_as_float(s[q4 & 1][e]),
+                                           __uint_as_float(s[q4 & 1][e + 1]));
+            }
+          } else {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) tmem_ld_32x32b_x32(s_cols + 32 * q4, s[q4]);
+            tc_wait_ld();
+            if (seen < 128) {
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4) mask32(s[q4], seen - 32 * q4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(s[0][e]);
+#pragma unroll
+            for (int e = 8; e < 128; e += 2)
+              mx8[(e >> 1) & 7] = fmax3f(mx8[(e >> 1) & 7], __uint_as_float(s[e >> 5][e & 31]),
+                                         __uint_as_float(s[e >> 5][(e + 1) & 31]));
+          }
           const float mx = fmax3f(fmax3f(mx8[0], mx8[1], mx8[2]), fmax3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
           const float m_row = mx * scale2;
-          if (j == w.j0) {
+          if (j == j0) {
             m_used = m_row;
           } else if (__any_sync(0xffffffffu, m_row > m_used + kRescaleThreshold)) {
             // taken by the whole warp: tcgen05.ld / st are warp-collective
@@ -503,20 +573,42 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           }
           const float m_sub = m_used == -INFINITY ? 0.f : m_used;  // nothing seen yet: all probabilities 0
           float rs8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if constexpr (C::QUANT) {
+            tmem_ld_32x32b_x32(s_cols, s[0]);
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), scale2, -m_sub));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), scale2, -m_sub));
-            if constexpr (!C::ONES) {
-              rs8[e & 7] += p0;
-              rs8[(e + 1) & 7] += p1;
+            for (int q4 = 0; q4 < 4; ++q4) {
+              tmem_arrived(s[q4 & 1]);
+              if (q4 < 3) tmem_ld_32x32b_x32(s_cols + 32 * (q4 + 1), s[(q4 + 1) & 1]);
+              uint32_t pr[16];
+              mask32(s[q4 & 1], seen - 32 * q4);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float p0 = ex2_approx(fmaf(__uint_as_float(s[q4 & 1][e]), scale2, -m_sub));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(s[q4 & 1][e + 1]), scale2, -m_sub));
+                if constexpr (!C::ONES) {
+                  rs8[e & 7] += p0;
+                  rs8[(e + 1) & 7] += p1;
+                }
+                pr[e >> 1] = pack_bf16(p0, p1);
+              }
+              tmem_st_32x32b_x16(s_cols + 16 * q4, pr);  // over scores that have been read
             }
-            s[e >> 6][(e >> 1) & 31] = pack_bf16(p0, p1);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 128; e += 2) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), scale2, -m_sub));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), scale2, -m_sub));
+              if constexpr (!C::ONES) {
+                rs8[e & 7] += p0;
+                rs8[(e + 1) & 7] += p1;
+              }
+              s[e >> 6][(e >> 1) & 31] = pack_bf16(p0, p1);
+            }
+            tmem_st_32x32b_x32(s_cols + 0, s[0]);
+            tmem_st_32x32b_x32(s_cols + 32, s[1]);
           }
           if constexpr (!C::ONES)
             l += ((rs8[0] + rs8[1]) + (rs8[2] + rs8[3])) + ((rs8[4] + rs8[5]) + (rs8[6] + rs8[7]));
-          tmem_st_32x32b_x32(s_cols + 0, s[0]);
-          tmem_st_32x32b_x32(s_cols + 32, s[1]);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -536,7 +628,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         __nv_bfloat16* dst = p.out + (long long)(w.it.seq.q0 + tok) * p.o_stride_t +
                              (long long)(w.it.kvh * p.group + head) * p.o_stride_h;
         // parts go to the workspace as [slot][column / 4][row]: a warp writes 512 contiguous bytes
-        const int slot = 2 * blockIdx.x + (w.u == u_begin ? 0 : 1);
+        const int slot = 2 * blockIdx.x + (part_no == 0 ? 0 : 1);
+        const bool whole = j1 - j0 == w.it.n_units;
         const int row = t * 128 + r;
         float4* part = reinterpret_cast<float4*>(ws.o) + (size_t)slot * (HD / 4) * kItemRows + row;
 #pragma unroll
@@ -549,7 +642,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free[t]);
           }
-          if (w.whole) {
+          if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 x;
@@ -567,9 +660,9 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                               __uint_as_float(ov[e + 3]));
           }
         }
-        if (!w.whole && live) ws.ml[(size_t)slot * kItemRows + row] = make_float2(m_used, l);
+        if (!whole && live) ws.ml[(size_t)slot * kItemRows + row] = make_float2(m_used, l);
       }
-      if (!leave_item(w, p.seqs, shape)) break;
+      if (!next_part_warp(w, p.seqs, shape, lane)) break;
     }
   }
 
