@@ -21,6 +21,10 @@
 //   x_j = s_j + log2 v_scale_j the weights 2^(x_j - m) that meet the codes have their maximum near 1 whatever
 //   the scales are, so fp16 holds them (the largest at 2^6, errors below 2^-30 of it), and the normaliser
 //   sums 2^(x_j - m) / v_scale_j in fp32.
+// Up to 16 rows each warp takes 16 of a unit's 64 tokens for all rows, and the four are joined at the end of
+// an item.  Above, up to 64, each warp takes a quarter of the rows for all tokens: it expands every code
+// itself, but holds a quarter of O (for all rows it spills), and nothing is joined.  64 rows of head_dim 64
+// over 8 int8 caches of 40000 tokens in all: SPLITTIME us, against 79 us split by tokens.
 // The running maximum is raised only when a score exceeds it by more than 2^8 (one vote per 16 tokens).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,6 +32,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -134,9 +139,11 @@ __device__ __forceinline__ uint32_t code_word(uint32_t w) {
   return FMT == KV_INT8 ? w ^ 0x80808080u : w;
 }
 
-template <int FMT, int HD, int NT>
+// NT: 8-row tiles per warp.  BY_ROWS: the warps split the rows, not the tokens.
+template <int FMT, int HD, int NT, bool BY_ROWS>
 struct DecodeCfg {
-  static constexpr int ROWS = 8 * NT;
+  static constexpr int ROWS = 8 * NT * (BY_ROWS ? kDecodeWarps : 1);
+  static constexpr int COPIES = BY_ROWS ? 1 : kDecodeWarps;  // of O, to be joined
   static constexpr int ELEM = FMT == KV_BF16 ? 2 : 1;
   static constexpr int ROW_BYTES = HD * ELEM;
   static constexpr int TILE = 16 * ROW_BYTES;                  // one warp's K (or V) of a unit
@@ -146,9 +153,9 @@ struct DecodeCfg {
   static constexpr float HEADROOM = FMT == KV_BF16 ? 0.f : 6.f;  // log2 of the largest weight (before lazy raises)
   static constexpr int RING = STAGES * STAGE;                  // per warp
   static constexpr int O_LD = HD + 4;                          // row stride of the merge buffer, in floats
-  static constexpr int MERGE = kDecodeWarps * ROWS * O_LD * 4;
+  static constexpr int MERGE = COPIES * ROWS * O_LD * 4;
   static constexpr int ML_OFF = kDecodeWarps * RING + MERGE;
-  static constexpr int SMEM = ML_OFF + kDecodeWarps * ROWS * 8;
+  static constexpr int SMEM = ML_OFF + COPIES * ROWS * 8;
 };
 
 // Byte offset of 16-byte chunk c of token row `tok` in a tile of 16 rows, arranged such that the fragment
@@ -172,10 +179,10 @@ __device__ __forceinline__ constexpr uint32_t pass_flip(int i) {
   return HD == 128 && IS_V ? ((2 * i) & 3) << 5 : 0;
 }
 
-template <int FMT, int HD, int NT>
+template <int FMT, int HD, int NT, bool BY_ROWS>
 __global__ void __launch_bounds__(kDecodeThreads)
     paged_decode_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
-  using C = DecodeCfg<FMT, HD, NT>;
+  using C = DecodeCfg<FMT, HD, NT, BY_ROWS>;
   constexpr bool QUANT = FMT != KV_BF16;
   constexpr int KS = HD / 16;  // k-steps of the scores, and 16-column tiles of O
   extern __shared__ __align__(128) uint8_t smem[];
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < C::STAGES; ++i) load_unit();
+  for (int i = 0; i < C::STAGES - (BY_ROWS ? 1 : 0); ++i) load_unit();
 
   // fragment addresses inside a stage (a stage starts on a multiple of 128 bytes: flipping bits 4 to 6 of the
   // sum flips them in the offset)
@@ -277,7 +284,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
   }
 
   const float scale2 = p.scale * kLog2e;
-  uint32_t slot_out = ring;
+  // Row tile t of this warp starts at row row0 + t * row_step: split by rows, the tiles go round the warps.
+  const int row0 = BY_ROWS ? warp * 8 : 0;
+  constexpr int row_step = BY_ROWS ? 8 * kDecodeWarps : 8;
+  const int copy0 = BY_ROWS ? 0 : warp * C::ROWS;
+  uint32_t slot_out = BY_ROWS ? smem_u32(smem) : ring;
+  int stage = 0;
   bool first = true;
   int unit = (int)(u_begin - it.start);
   while (true) {  // one item, or the part of it in this block's range
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     float q_unit[NT][2];  // 8-bit: what the scores of rows 2 j and 2 j + 1 are multiplied by
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int r = 8 * t + n;
+      const int r = row0 + t * row_step + n;
       const bool ok = r < rows;
       const __nv_bfloat16* src = p.q + (long long)(it.seq.q0 + tok0 + r / p.group) * p.q_stride_t +
                                  (long long)(it.kvh * p.group + r % p.group) * p.q_stride_h;
@@ -346,172 +358,198 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
     for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
 
-    for (int c = 0; c < seg; ++c, ++unit) {
-      cp_async_wait<C::STAGES - 1>();
-      __syncwarp();
-      const int t0 = unit * 64 + 16 * warp;
-      if (t0 < visible) {
-        const uint32_t ka = slot_out + k_frag, va = slot_out + v_frag;
-        float s[NT][4];
+    // 16 tokens from t0 on, at `tile` in shared memory, against the first N row tiles
+    auto step = [&](auto n_tiles, uint32_t tile, int t0) {
+      constexpr int N = decltype(n_tiles)::value;
+      const uint32_t ka = tile + k_frag, va = tile + v_frag;
+      float s[N][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        if constexpr (!QUANT) {
+      for (int t = 0; t < N; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      if constexpr (!QUANT) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t a[4];
+          ldsm_x4((ka ^ (((2 * ks) & 7) << 4)) + (ks >> 2) * 128, a);
+#pragma unroll
+          for (int t = 0; t < N; ++t) mma_16816<false>(s[t], a, qf[t][ks][0], qf[t][ks][1]);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < HD / 64; ++g) {
+          uint32_t lo[4], hi[4];
+          lds128(ka ^ (g << 6), lo);
+          lds128((ka ^ (g << 6)) + 8 * HD, hi);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
             uint32_t a[4];
-            ldsm_x4((ka ^ (((2 * ks) & 7) << 4)) + (ks >> 2) * 128, a);
+            codes_to_f16<FMT>(code_word<FMT>(lo[x]), a[0], a[2]);
+            codes_to_f16<FMT>(code_word<FMT>(hi[x]), a[1], a[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16816<false>(s[t], a, qf[t][ks][0], qf[t][ks][1]);
-          }
-        } else {
-#pragma unroll
-          for (int g = 0; g < HD / 64; ++g) {
-            uint32_t lo[4], hi[4];
-            lds128(ka ^ (g << 6), lo);
-            lds128((ka ^ (g << 6)) + 8 * HD, hi);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t a[4];
-              codes_to_f16<FMT>(code_word<FMT>(lo[x]), a[0], a[2]);
-              codes_to_f16<FMT>(code_word<FMT>(hi[x]), a[1], a[3]);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) mma_16816<true>(s[t], a, qf[t][4 * g + x][0], qf[t][4 * g + x][1]);
-            }
-          }
-        }
-        // scores in log2 units; 8-bit: plus log2 of v_scale, with w = 1 / v_scale for the normaliser
-        float w0 = 1.f, w1 = 1.f;
-        if constexpr (QUANT) {
-          const uint32_t sa = slot_out + 2 * C::TILE + n * 4;
-          const float k0 = lds32f(sa), k1 = lds32f(sa + 32), v0 = lds32f(sa + 64), v1 = lds32f(sa + 96);
-          // a scale of 0 (all codes 0) counts as 2^-100; a NaN stays one
-          const float x0 = lg2_approx(fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
-          const float x1 = lg2_approx(fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
-          w0 = ex2_approx(-x0);
-          w1 = ex2_approx(-x1);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            s[t][0] = fmaf(s[t][0], k0 * q_unit[t][0], x0);
-            s[t][1] = fmaf(s[t][1], k0 * q_unit[t][1], x0);
-            s[t][2] = fmaf(s[t][2], k1 * q_unit[t][0], x1);
-            s[t][3] = fmaf(s[t][3], k1 * q_unit[t][1], x1);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] *= scale2;
-        }
-        if (t0 + 16 > all_see) {  // a row that does not exist is masked like the last one
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int lim = min(base_pos + (8 * t + 2 * j + e) / p.group + 1, visible);
-              if (t0 + n >= lim) s[t][e] = -INFINITY;
-              if (t0 + n + 8 >= lim) s[t][2 + e] = -INFINITY;
-            }
-        }
-        bool raise = false;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise || fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(s[t][e], s[t][2 + e]);
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float m_new = fmaxf(m[t][e], mx);
-              const float alpha = m_new == m[t][e] ? 1.f : ex2_approx(m[t][e] - m_new);
-              m[t][e] = m_new;
-              l[t][e] *= alpha;
-#pragma unroll
-              for (int i = 0; i < KS; ++i) {
-                o[i][t][e] *= alpha;
-                o[i][t][2 + e] *= alpha;
-              }
-            }
-        }
-        uint32_t pf[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          // nothing seen yet: all weights 0
-          const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0] - C::HEADROOM;
-          const float m1 = m[t][1] == -INFINITY ? 0.f : m[t][1] - C::HEADROOM;
-          const float p0 = ex2_approx(s[t][0] - m0), p1 = ex2_approx(s[t][1] - m1);
-          const float p2 = ex2_approx(s[t][2] - m0), p3 = ex2_approx(s[t][3] - m1);
-          l[t][0] += QUANT ? fmaf(p0, w0, p2 * w1) : p0 + p2;
-          l[t][1] += QUANT ? fmaf(p1, w0, p3 * w1) : p1 + p3;
-          // rounded for the product with V (bf16: half a step of 2^-8 relative for each probability)
-          pf[t][0] = transpose_8x8(pack_pair<QUANT>(p0, p1));
-          pf[t][1] = transpose_8x8(pack_pair<QUANT>(p2, p3));
-        }
-        if constexpr (!QUANT) {
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            uint32_t a[4];
-            ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
-          }
-        } else {
-          // tile i: O's rows n and n + 8 are columns n * HD / 8 + 2 i and + 1 of V; words of tokens
-          // 2 j, 2 j + 1, 2 j + 8, 2 j + 9
-          constexpr int W = HD / 32;
-          uint32_t w[4][W];
-          if constexpr (HD == 128) {
-            lds128(va, w[0]);
-            lds128(va + 128, w[1]);
-            lds128(va + 1024, w[2]);
-            lds128(va + 1152, w[3]);
-          } else {
-            lds64(va, w[0][0], w[0][1]);
-            lds64(va ^ 64, w[1][0], w[1][1]);
-            lds64(va + 512, w[2][0], w[2][1]);
-            lds64((va ^ 64) + 512, w[3][0], w[3][1]);
-          }
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const int k = i >> 1;
-            const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-            uint32_t a[4];
-            codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[0][k], w[1][k], sel)), a[0], a[1]);
-            codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[2][k], w[3][k], sel)), a[2], a[3]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16816<true>(o[i][t], a, pf[t][0], pf[t][1]);
+            for (int t = 0; t < N; ++t) mma_16816<true>(s[t], a, qf[t][4 * g + x][0], qf[t][4 * g + x][1]);
           }
         }
       }
-      __syncwarp();  // every lane has read the stage before it is loaded again
-      load_unit();
-      slot_out = slot_out + C::STAGE == ring + C::RING ? ring : slot_out + C::STAGE;
+      // scores in log2 units; 8-bit: plus log2 of v_scale, with w = 1 / v_scale for the normaliser
+      float w0 = 1.f, w1 = 1.f;
+      if constexpr (QUANT) {
+        const uint32_t sa = tile + 2 * C::TILE + n * 4;
+        const float k0 = lds32f(sa), k1 = lds32f(sa + 32), v0 = lds32f(sa + 64), v1 = lds32f(sa + 96);
+        // a scale of 0 (all codes 0) counts as 2^-100; a NaN stays one
+        const float x0 = lg2_approx(fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
+        const float x1 = lg2_approx(fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
+        w0 = ex2_approx(-x0);
+        w1 = ex2_approx(-x1);
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+          s[t][0] = fmaf(s[t][0], k0 * q_unit[t][0], x0);
+          s[t][1] = fmaf(s[t][1], k0 * q_unit[t][1], x0);
+          s[t][2] = fmaf(s[t][2], k1 * q_unit[t][0], x1);
+          s[t][3] = fmaf(s[t][3], k1 * q_unit[t][1], x1);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] *= scale2;
+      }
+      if (t0 + 16 > all_see) {  // a row that does not exist is masked like the last one
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int lim = min(base_pos + (row0 + t * row_step + 2 * j + e) / p.group + 1, visible);
+            if (t0 + n >= lim) s[t][e] = -INFINITY;
+            if (t0 + n + 8 >= lim) s[t][2 + e] = -INFINITY;
+          }
+      }
+      bool raise = false;
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+        raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise || fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[t][e], s[t][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m[t][e], mx);
+            const float alpha = m_new == m[t][e] ? 1.f : ex2_approx(m[t][e] - m_new);
+            m[t][e] = m_new;
+            l[t][e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              o[i][t][e] *= alpha;
+              o[i][t][2 + e] *= alpha;
+            }
+          }
+      }
+      uint32_t pf[N][2];
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        // nothing seen yet: all weights 0
+        const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0] - C::HEADROOM;
+        const float m1 = m[t][1] == -INFINITY ? 0.f : m[t][1] - C::HEADROOM;
+        const float p0 = ex2_approx(s[t][0] - m0), p1 = ex2_approx(s[t][1] - m1);
+        const float p2 = ex2_approx(s[t][2] - m0), p3 = ex2_approx(s[t][3] - m1);
+        l[t][0] += QUANT ? fmaf(p0, w0, p2 * w1) : p0 + p2;
+        l[t][1] += QUANT ? fmaf(p1, w0, p3 * w1) : p1 + p3;
+        // rounded for the product with V (bf16: half a step of 2^-8 relative for each probability)
+        pf[t][0] = transpose_8x8(pack_pair<QUANT>(p0, p1));
+        pf[t][1] = transpose_8x8(pack_pair<QUANT>(p2, p3));
+      }
+      if constexpr (!QUANT) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          uint32_t a[4];
+          ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
+#pragma unroll
+          for (int t = 0; t < N; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
+        }
+      } else {
+        // tile i: O's rows n and n + 8 are columns n * HD / 8 + 2 i and + 1 of V; words of tokens
+        // 2 j, 2 j + 1, 2 j + 8, 2 j + 9
+        constexpr int W = HD / 32;
+        uint32_t w[4][W];
+        if constexpr (HD == 128) {
+          lds128(va, w[0]);
+          lds128(va + 128, w[1]);
+          lds128(va + 1024, w[2]);
+          lds128(va + 1152, w[3]);
+        } else {
+          lds64(va, w[0][0], w[0][1]);
+          lds64(va ^ 64, w[1][0], w[1][1]);
+          lds64(va + 512, w[2][0], w[2][1]);
+          lds64((va ^ 64) + 512, w[3][0], w[3][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          const int k = i >> 1;
+          const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+          uint32_t a[4];
+          codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[0][k], w[1][k], sel)), a[0], a[1]);
+          codes_to_f16<FMT>(code_word<FMT>(__byte_perm(w[2][k], w[3][k], sel)), a[2], a[3]);
+#pragma unroll
+          for (int t = 0; t < N; ++t) mma_16816<true>(o[i][t], a, pf[t][0], pf[t][1]);
+        }
+      }
+    };
+    const int live_tiles = min(NT, max(0, (rows - row0 + row_step - 1) / row_step));
+
+    for (int c = 0; c < seg; ++c, ++unit) {
+      if constexpr (BY_ROWS) {
+        cp_async_wait<C::STAGES - 2>();
+        __syncthreads();  // the stage is there for all warps, and all have read the one before
+        load_unit();
+      } else {
+        cp_async_wait<C::STAGES - 1>();
+        __syncwarp();
+      }
+#pragma unroll 1
+      for (int x = 0; x < (BY_ROWS ? kDecodeWarps : 1); ++x) {
+        const uint32_t tile = slot_out + (BY_ROWS ? x * C::RING : 0);
+        const int t0 = unit * 64 + 16 * (BY_ROWS ? x : warp);
+        if (t0 >= visible) break;
+        if (NT > 1 && live_tiles < NT) {
+          if (live_tiles > 0) step(std::integral_constant<int, 1>(), tile, t0);
+        } else if (NT > 1 || !BY_ROWS || live_tiles > 0) {
+          step(std::integral_constant<int, NT>(), tile, t0);
+        }
+      }
+      if constexpr (!BY_ROWS) {
+        __syncwarp();  // every lane has read the stage before it is loaded again
+        load_unit();
+      }
+      slot_out += C::STAGE;
+      if (++stage == C::STAGES) {
+        stage = 0;
+        slot_out -= C::RING;
+      }
     }
 
-    // ---- join the four warps
+    // ---- join the warps
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], x);
-        if (n == 0) ml_smem[warp * C::ROWS + 8 * t + 2 * j + e] = make_float2(m[t][e], l[t][e]);
+        if (n == 0) ml_smem[copy0 + row0 + t * row_step + 2 * j + e] = make_float2(m[t][e], l[t][e]);
       }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = 8 * t + 2 * j + e;
+        const int r = row0 + t * row_step + 2 * j + e;
         if (r >= rows) continue;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kDecodeWarps; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
+        for (int w = 0; w < C::COPIES; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
         const float f = m[t][e] == mx ? 1.f : ex2_approx(m[t][e] - mx);
-        float* dst = merge + (warp * C::ROWS + r) * C::O_LD;
+        float* dst = merge + (copy0 + r) * C::O_LD;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           const int d0 = QUANT ? n * (HD / 8) + 2 * i : 16 * i + n;
@@ -526,10 +564,10 @@ __global__ void __launch_bounds__(kDecodeThreads)
       const int r = x / (HD / 4), d = (x % (HD / 4)) * 4;
       float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kDecodeWarps; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
+      for (int w = 0; w < C::COPIES; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kDecodeWarps; ++w) {
+      for (int w = 0; w < C::COPIES; ++w) {
         const float2 q = ml_smem[w * C::ROWS + r];
         sum += q.x == mx ? q.y : q.y * ex2_approx(q.x - mx);
         const float4 v = *reinterpret_cast<const float4*>(merge + (w * C::ROWS + r) * C::O_LD + d);
@@ -560,12 +598,14 @@ __global__ void __launch_bounds__(kDecodeThreads)
 
 // Joins the parts of items that lie in more than one block's range.  Block x + 1 of the attention kernel
 // starts inside an item, or does not; the first block that does joins the item.  WARPS_PER_ROW warps share
-// the parts of a row; ROWS rows per part.
+// the parts of a row; ROWS rows per part.  Few and large blocks: most find nothing to do, and a launch of one
+// block per row (28000 for 64 rows) took 25 us for that alone.
+constexpr int kJoinThreads = 256;
 template <int HD, int ROWS, int WARPS_PER_ROW>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinThreads)
     paged_join_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
   pdl_wait_and_release();
-  constexpr int ROWS_AT_ONCE = 4 / WARPS_PER_ROW;
+  constexpr int ROWS_AT_ONCE = kJoinThreads / 32 / WARPS_PER_ROW;
   constexpr int V = HD / 32;  // columns per lane
   const long long total = ws.total[0];
   const int blocks = (int)ws.total[1];
@@ -584,8 +624,8 @@ __global__ void __launch_bounds__(128)
   const int rows = min(shape.tile_tokens, seq.qn - tok0) * p.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = warp % WARPS_PER_ROW;
-  __shared__ float part[4][HD];
-  __shared__ float part_l[4];
+  __shared__ float part[kJoinThreads / 32][HD];
+  __shared__ float part_l[kJoinThreads / 32];
   for (int r0 = blockIdx.y * ROWS_AT_ONCE; r0 < rows; r0 += gridDim.y * ROWS_AT_ONCE) {
     const int r = r0 + warp / WARPS_PER_ROW;
     const bool live = r < rows;
@@ -598,7 +638,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
     if (live) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = sub; i < parts; i += WARPS_PER_ROW) {
         const size_t at = (size_t)slot(i) * ROWS + r;
         const float2 q = ws.ml[at];
@@ -646,16 +686,16 @@ __global__ void __launch_bounds__(128)
 }
 
 // Blocks of the kernel that the current device holds at once.
-template <int FMT, int HD, int NT>
+template <int FMT, int HD, int NT, bool BY_ROWS>
 int decode_blocks() {
-  using C = DecodeCfg<FMT, HD, NT>;
+  using C = DecodeCfg<FMT, HD, NT, BY_ROWS>;
   static std::atomic<int> cached[64];
   int dev = 0;
   B200_CUDA_CHECK(cudaGetDevice(&dev));
   B200_CHECK(dev >= 0 && dev < 64, "device index out of range");
   int n = cached[dev].load(std::memory_order_acquire);
   if (n == 0) {
-    auto* kernel = paged_decode_kernel<FMT, HD, NT>;
+    auto* kernel = paged_decode_kernel<FMT, HD, NT, BY_ROWS>;
     B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     int per_sm = 0;
     B200_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kDecodeThreads, C::SMEM));
@@ -666,14 +706,17 @@ int decode_blocks() {
   return n;
 }
 
-template <int FMT, int HD, int NT>
+template <int FMT, int HD, int NT, bool BY_ROWS>
 void launch_decode(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
-  using C = DecodeCfg<FMT, HD, NT>;
-  const int blocks = decode_blocks<FMT, HD, NT>();
+  using C = DecodeCfg<FMT, HD, NT, BY_ROWS>;
+  const int blocks = decode_blocks<FMT, HD, NT, BY_ROWS>();
   const PagedWorkspace ws = paged_workspace(alloc(paged_workspace_bytes(blocks, C::ROWS, HD)), blocks, C::ROWS);
   const PagedShape shape{std::max(1, C::ROWS / p.group), kUnitLog2, p.pool.kv_heads};
-  launch_k(paged_decode_kernel<FMT, HD, NT>, dim3(blocks), dim3(kDecodeThreads), C::SMEM, s, 1, p, shape, ws);
-  launch_k(paged_join_kernel<HD, C::ROWS, 4>, dim3(blocks - 1, C::ROWS), dim3(128), 0, s, 1, p, shape, ws);
+  launch_k(paged_decode_kernel<FMT, HD, NT, BY_ROWS>, dim3(blocks), dim3(kDecodeThreads), C::SMEM, s, 1, p, shape, ws);
+  // one row has many parts when there are few rows, and few when there are many
+  constexpr int WARPS_PER_ROW = C::ROWS <= 16 ? 4 : 1;
+  launch_k(paged_join_kernel<HD, C::ROWS, WARPS_PER_ROW>, dim3(blocks - 1, 4), dim3(kJoinThreads), 0, s, 1, p, shape,
+           ws);
   B200_CUDA_CHECK(cudaGetLastError());
   count_launch(2);
 }
@@ -682,13 +725,13 @@ template <int FMT, int HD>
 void launch_rows(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
   const long long rows = (long long)p.seqs.max_q * p.group;
   if (rows <= 8)
-    launch_decode<FMT, HD, 1>(p, alloc, s);
+    launch_decode<FMT, HD, 1, false>(p, alloc, s);
   else if (rows <= 16)
-    launch_decode<FMT, HD, 2>(p, alloc, s);
+    launch_decode<FMT, HD, 2, false>(p, alloc, s);
   else if (rows <= 32)
-    launch_decode<FMT, HD, 4>(p, alloc, s);
-  else if (HD == 64 && rows <= 64)
-    launch_decode<FMT, 64, 8>(p, alloc, s);
+    launch_decode<FMT, HD, 1, true>(p, alloc, s);
+  else if (rows <= 64)
+    launch_decode<FMT, HD, 2, true>(p, alloc, s);
   else
     paged_attention_chunk(p, alloc, s);
 }
