@@ -1,10 +1,12 @@
 // Python bindings of the serving kernels: paged key/value cache, attention over it, logit adjustment.
 // Shapes and types are checked before anything touches a device.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <climits>
+#include <cmath>
 #include <optional>
 #include <vector>
 
@@ -137,8 +139,9 @@ void check_devices(const Tensor& first, const Tensor& k, const Tensor& v, const 
 
 cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-void kv_cache_write(Tensor k_pages, Tensor v_pages, std::optional<Tensor> k_scale, std::optional<Tensor> v_scale,
-                    Tensor k, Tensor v, Tensor table, Tensor lens, std::optional<Tensor> starts) {
+void kv_cache_write(const Tensor& k_pages, const Tensor& v_pages, const std::optional<Tensor>& k_scale,
+                    const std::optional<Tensor>& v_scale, const Tensor& k, const Tensor& v, const Tensor& table,
+                    const Tensor& lens, const std::optional<Tensor>& starts) {
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
   const RowStrides sk = check_rows(k, -1, pool.kv_heads, pool.head_dim, false, "k");
   const RowStrides sv = check_rows(v, k.size(0), pool.kv_heads, pool.head_dim, false, "v");
@@ -151,28 +154,27 @@ void kv_cache_write(Tensor k_pages, Tensor v_pages, std::optional<Tensor> k_scal
                        reinterpret_cast<const __nv_bfloat16*>(v.data_ptr()), sk.t, sk.h, sv.t, sv.h, cur_stream());
 }
 
-void kv_cache_read(Tensor k_pages, Tensor v_pages, std::optional<Tensor> k_scale, std::optional<Tensor> v_scale,
-                   Tensor k, Tensor v, Tensor table, Tensor lens, std::optional<Tensor> starts) {
+std::tuple<Tensor, Tensor> kv_cache_read(const Tensor& k_pages, const Tensor& v_pages,
+                                         const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                                         const Tensor& table, const Tensor& lens, const std::optional<Tensor>& starts,
+                                         int64_t total, at::ScalarType type) {
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
-  for (const Tensor* t : {&k, &v})
-    TORCH_CHECK(t->dim() == 3 && t->size(1) == pool.kv_heads && t->size(2) == pool.head_dim &&
-                    t->size(0) == k.size(0) && t->is_contiguous() && t->scalar_type() == k.scalar_type(),
-                "k and v must be contiguous [tokens, kv_heads, head_dim] tensors of one dtype");
-  TORCH_CHECK(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat,
-              "the cache is read as bfloat16 or float32");
-  check_aligned(k, "k");
-  check_aligned(v, "v");
-  const b200::PagedSeqs seqs = check_seqs(k_pages, table, lens, starts, k.size(0), INT_MAX);
-  check_device(k, k, "k");
-  check_device(v, k, "v");
-  check_devices(k, k_pages, v_pages, k_scale, v_scale, table, lens, starts);
-  c10::cuda::CUDAGuard g(k.device());
-  b200::kv_cache_read(seqs, pool, k.data_ptr(), v.data_ptr(), k.scalar_type() == at::kFloat, cur_stream());
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kFloat, "the cache is read as bfloat16 or float32");
+  TORCH_CHECK(total >= 0, "total must not be negative");
+  const b200::PagedSeqs seqs = check_seqs(k_pages, table, lens, starts, total, INT_MAX);
+  check_devices(k_pages, k_pages, v_pages, k_scale, v_scale, table, lens, starts);
+  c10::cuda::CUDAGuard g(k_pages.device());
+  const auto options = k_pages.options().dtype(type);
+  Tensor k = at::empty({total, pool.kv_heads, pool.head_dim}, options);
+  Tensor v = at::empty({total, pool.kv_heads, pool.head_dim}, options);
+  b200::kv_cache_read(seqs, pool, k.data_ptr(), v.data_ptr(), type == at::kFloat, cur_stream());
+  return {k, v};
 }
 
-void paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, std::optional<Tensor> k_scale,
-                     std::optional<Tensor> v_scale, Tensor out, Tensor table, Tensor lens,
-                     std::optional<Tensor> starts, int64_t max_q, double scale) {
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                       const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                       const std::optional<Tensor>& out_, const Tensor& table, const Tensor& lens,
+                       const std::optional<Tensor>& starts, int64_t max_q, std::optional<double> scale_) {
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
   TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", shape(q));
   const int64_t heads = q.size(1);
@@ -180,16 +182,21 @@ void paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, std::optional<Ten
               ") must be a multiple of kv_heads (", std::to_string(pool.kv_heads), ")");
   TORCH_CHECK(heads / pool.kv_heads <= 128, "more than 128 query heads share a kv head");
   const RowStrides sq = check_rows(q, -1, heads, pool.head_dim, false, "q");
-  const RowStrides so = check_rows(out, q.size(0), heads, pool.head_dim, true, "out");
-  TORCH_CHECK(!out.is_alias_of(q) && !out.is_alias_of(k_pages) && !out.is_alias_of(v_pages),
-              "out must not share memory with q or the pages");
+  if (out_.has_value()) {
+    check_rows(*out_, q.size(0), heads, pool.head_dim, true, "out");
+    TORCH_CHECK(!out_->is_alias_of(q) && !out_->is_alias_of(k_pages) && !out_->is_alias_of(v_pages),
+                "out must not share memory with q or the pages");
+  }
   TORCH_CHECK(max_q >= 1 && max_q <= INT_MAX, "max_q_len must be at least 1");
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)pool.head_dim);
   TORCH_CHECK(scale > 0.0 && scale <= 1e30, "scale must be positive and finite");
   const b200::PagedSeqs seqs = check_seqs(k_pages, table, lens, starts, q.size(0), max_q);
   check_device(q, q, "q");
-  check_device(out, q, "out");
+  if (out_.has_value()) check_device(*out_, q, "out");
   check_devices(q, k_pages, v_pages, k_scale, v_scale, table, lens, starts);
   c10::cuda::CUDAGuard g(q.device());
+  Tensor out = out_.has_value() ? *out_ : at::empty(q.sizes(), q.options());
+  const RowStrides so = check_rows(out, q.size(0), heads, pool.head_dim, true, "out");
   b200::PagedAttnParams p{};
   p.seqs = seqs;
   p.pool = pool;
@@ -202,14 +209,16 @@ void paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, std::optional<Ten
   p.heads = (int)heads;
   p.group = (int)(heads / pool.kv_heads);
   p.scale = (float)scale;
-  Tensor workspace;  // from PyTorch's allocator: reused in stream order, private to a graph that captures the call
+  // from PyTorch's allocator: reused in stream order, private to a graph that captures the call
+  c10::DataPtr workspace;
   b200::paged_attention(
       p,
       [&](size_t bytes) {
-        workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-        return workspace.data_ptr();
+        workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+        return workspace.get();
       },
       cur_stream());
+  return out;
 }
 
 // Host-only view of how the attention kernels divide their work (CPU tensors, no GPU needed): per block and
@@ -262,21 +271,24 @@ void check_per_row(const std::optional<Tensor>& t, const Tensor& logits, at::Sca
               " must be contiguous ", type, " [", std::to_string(logits.size(0)), "]");
 }
 
-void adjust_logits(Tensor logits, Tensor out, std::optional<Tensor> history, std::optional<Tensor> history_lens,
-                   std::optional<Tensor> prompt_lens, std::optional<Tensor> repetition,
-                   std::optional<Tensor> frequency, std::optional<Tensor> presence, std::optional<Tensor> bias,
-                   std::optional<Tensor> allowed) {
+Tensor adjust_logits(const Tensor& logits, const std::optional<Tensor>& out_, const std::optional<Tensor>& history,
+                     const std::optional<Tensor>& history_lens, const std::optional<Tensor>& prompt_lens,
+                     const std::optional<Tensor>& repetition, const std::optional<Tensor>& frequency,
+                     const std::optional<Tensor>& presence, const std::optional<Tensor>& bias,
+                     const std::optional<Tensor>& allowed) {
   TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
               "logits must be [batch, vocab] with unit column stride");
-  TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() &&
-                  (out.size(1) <= 1 || out.stride(1) == 1),
-              "out must have the logits' shape and dtype and unit column stride");
   const int64_t batch = logits.size(0), vocab = logits.size(1);
   TORCH_CHECK(vocab <= INT_MAX - 65536 && batch <= 1 << 20, "logits: too many rows or columns");
-  TORCH_CHECK(batch <= 1 || out.stride(0) >= vocab, "out rows must not overlap");
-  if (out.is_alias_of(logits))
-    TORCH_CHECK(out.data_ptr() == logits.data_ptr() && (batch <= 1 || out.stride(0) == logits.stride(0)),
-                "out must be the logits themselves or not share memory with them");
+  if (out_.has_value()) {
+    TORCH_CHECK(out_->sizes() == logits.sizes() && out_->scalar_type() == logits.scalar_type() &&
+                    (vocab <= 1 || out_->stride(1) == 1),
+                "out must have the logits' shape and dtype and unit column stride");
+    TORCH_CHECK(batch <= 1 || out_->stride(0) >= vocab, "out rows must not overlap");
+    if (out_->is_alias_of(logits))
+      TORCH_CHECK(out_->data_ptr() == logits.data_ptr() && (batch <= 1 || out_->stride(0) == logits.stride(0)),
+                  "out must be the logits themselves or not share memory with them");
+  }
   b200::LogitsParams p{};
   const at::ScalarType type = logits.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat,
@@ -313,7 +325,7 @@ void adjust_logits(Tensor logits, Tensor out, std::optional<Tensor> history, std
     p.allowed_stride = allowed->dim() == 2 ? allowed->stride(0) : 0;
   }
   check_device(logits, logits, "logits");
-  check_device(out, logits, "out");
+  if (out_.has_value()) check_device(*out_, logits, "out");
   const std::pair<const std::optional<Tensor>*, const char*> rest[] = {
       {&history, "history"},   {&history_lens, "history_lens"}, {&prompt_lens, "prompt_lens"},
       {&repetition, "repetition_penalty"}, {&frequency, "frequency_penalty"}, {&presence, "presence_penalty"},
@@ -321,6 +333,7 @@ void adjust_logits(Tensor logits, Tensor out, std::optional<Tensor> history, std
   for (const auto& [t, name] : rest)
     if (t->has_value()) check_device(**t, logits, name);
   c10::cuda::CUDAGuard g(logits.device());
+  Tensor out = out_.has_value() ? *out_ : at::empty(logits.sizes(), logits.options());
   p.logits = logits.data_ptr();
   p.out = out.data_ptr();
   p.stride = logits.stride(0);
@@ -338,13 +351,20 @@ void adjust_logits(Tensor logits, Tensor out, std::optional<Tensor> history, std
     p.presence = presence.has_value() ? presence->data_ptr<float>() : nullptr;
   }
   b200::adjust_logits(p, cur_stream());
+  return out;
 }
 
 }  // namespace
 
 void bind_serving(pybind11::module_& m) {
   m.def("kv_cache_write", &kv_cache_write);
-  m.def("kv_cache_read", &kv_cache_read);
+  m.def("kv_cache_read",
+        [](const Tensor& k, const Tensor& v, const std::optional<Tensor>& ks, const std::optional<Tensor>& vs,
+           const Tensor& table, const Tensor& lens, const std::optional<Tensor>& starts, int64_t total,
+           const py::object& dtype) {
+          return kv_cache_read(k, v, ks, vs, table, lens, starts, total,
+                               torch::python::detail::py_object_to_dtype(dtype));
+        });
   m.def("paged_attention", &paged_attention);
   m.def("paged_schedule", &paged_schedule);
   m.def("adjust_logits", &adjust_logits);

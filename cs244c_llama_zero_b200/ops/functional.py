@@ -288,8 +288,8 @@ class KVPages(NamedTuple):
     v_scale: Optional[torch.Tensor] = None
 
 
-def _no_backward(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_backward(name: str, tensor: torch.Tensor) -> None:
+    if tensor.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
 
 
@@ -298,8 +298,9 @@ def kv_cache_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     """Write the new tokens' keys and values (bf16 ``[tokens, kv_heads, head_dim]``, any row strides that
     are multiples of 8) to their places in the cache, quantising them if the pages are 8-bit.  The pages
     that take new tokens must belong to one sequence each.  Rows of no sequence are ignored."""
-    _no_backward("kv_cache_write", k, v)
-    _ext().kv_cache_write(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, block_table, kv_lens, q_starts)
+    _no_backward("kv_cache_write", k)
+    _no_backward("kv_cache_write", v)
+    _ext().kv_cache_write(*pages, k, v, block_table, kv_lens, q_starts)
 
 
 def kv_cache_read(pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -312,11 +313,7 @@ def kv_cache_read(pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tens
         if q_starts is not None:
             raise ValueError("kv_cache_read: total (the number of rows) is needed with q_starts")
         total = block_table.shape[0]
-    shape = (total, pages.k.shape[1], pages.k.shape[3])
-    k = torch.empty(shape, dtype=dtype, device=pages.k.device)
-    v = torch.empty(shape, dtype=dtype, device=pages.k.device)
-    _ext().kv_cache_read(pages.k, pages.v, pages.k_scale, pages.v_scale, k, v, block_table, kv_lens, q_starts)
-    return k, v
+    return _ext().kv_cache_read(*pages, block_table, kv_lens, q_starts, total, dtype)
 
 
 def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -337,11 +334,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         if q_starts is not None:
             raise ValueError("paged_attention: max_q_len is needed with q_starts")
         max_q_len = 1
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _ext().paged_attention(q, pages.k, pages.v, pages.k_scale, pages.v_scale, out, block_table, kv_lens, q_starts,
-                           max_q_len, q.shape[-1] ** -0.5 if scale is None else scale)
-    return out
+    return _ext().paged_attention(q, *pages, out, block_table, kv_lens, q_starts, max_q_len, scale)
 
 
 # ------------------------------------------------------------------------------ logits
@@ -362,11 +355,8 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     ``t % 32`` of word ``t // 32``) is 0 become ``-inf``.  Computed in fp32.  ``out`` may be ``logits``.
     A token id outside the vocabulary is skipped and recorded (``ops.check_device_errors()``)."""
     _no_backward("adjust_logits", logits)
-    if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _ext().adjust_logits(logits, out, history, history_lens, prompt_lens, repetition_penalty, frequency_penalty,
-                         presence_penalty, bias, allowed)
-    return out
+    return _ext().adjust_logits(logits, out, history, history_lens, prompt_lens, repetition_penalty,
+                                frequency_penalty, presence_penalty, bias, allowed)
 
 
 # ------------------------------------------------------------------------------ transformer block

@@ -353,7 +353,7 @@ def _logit_tol(want, logits, dtype, length):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("batch,vocab,length", [(1, 1, 3), (2, 31, 0), (3, 1000, 50), (2, 8191, 700), (2, 32000, 300),
-                                                (1, 9999, 1)])
+                                                (1, 9999, 1), (2, 5000, 3000), (2, 600, 5000)])
 def test_logits(F, dtype, batch, vocab, length):
     logits, history, lens, prompts, rep, freq, pres, bias, allowed = _logit_case(batch, vocab, dtype, length, vocab)
     cu = [t.cuda() for t in (logits, history, lens, prompts, rep, freq, pres, bias, allowed)]
