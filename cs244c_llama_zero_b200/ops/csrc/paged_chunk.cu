@@ -10,8 +10,13 @@
 //      per page and 64 columns); warp 1 issues the MMAs; warp 2 zeroes V's rows behind the last visible token.
 //   1, 2: softmax of tile A and B, one thread per row, as in the training forward kernel: scores from tensor
 //      memory, probabilities back into the same columns as the A operand of the PV product, lazy rescaling of O.
-//   3 (8-bit pages only): expands codes into the shared-memory tiles as bf16 (code * scale, rounded once: half a
-//      step of 2^-8 relative, as for unquantised bf16 keys and values).
+//   3 (8-bit pages only): loads Q, and expands codes into the shared-memory tiles; see below.
+// With 8-bit pages the products are taken in fp16, whose 11 bits lose nothing next to the result's 8: a row of q is
+// scaled by a power of two to a maximum in [1, 2), and code * scale of K and of V by one for each unit of 128
+// tokens (to a maximum in (2^14, 2^15]), then rounded once (2^-12 relative).  K's power multiplies the unit's
+// scores.  V's, 2^e, goes into the exponent: the weights are 2^(s_j + e - m), with the running maximum m taken
+// over s_j + e and 2^6 of headroom, and the normaliser sums them times 2^-e.  Rounding code * scale to bf16
+// instead cost two bits of the result.
 // MMA order: S_A(0) S_B(0) | PV_A(j) S_A(j+1) PV_B(j) S_B(j+1) | ...
 //
 // Masking is by selection (a masked score becomes -inf whatever K holds), and V's rows behind the last visible
@@ -38,6 +43,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr float kHeadroom = 6.0f;          // 8-bit: log2 of the largest weight (before lazy raises)
 constexpr int kItemRows = 256;
 
 template <int FMT, int HD>
@@ -57,13 +63,14 @@ struct ChunkCfg {
   static constexpr int REGS_NEEDED = QUANT ? 0 : 128 * REGS_LOW + 256 * REGS_HIGH;
   static_assert(REGS_NEEDED <= THREADS * LAUNCH_REGS, "register split over budget");
   // hd 64: row sums from the tensor cores, by a block of ones behind V (see the training forward kernel)
-  static constexpr bool ONES = (HD == 64);
+  static constexpr bool ONES = (HD == 64) && !QUANT;  // (8-bit: the sums are weighted for each unit)
   static constexpr int O_COLS = ONES ? HD + 16 : HD;
   static constexpr int STAGE_BYTES = (ONES ? 3 : 2) * TILE_BYTES;
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = Q_BUFS * 2 * TILE_BYTES;
   static constexpr int BAR_OFF = KV_OFF + STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
+  static constexpr int UNIT_OFF = BAR_OFF + 256;  // 8-bit: powers of two of Q's rows, K's and V's units
+  static constexpr int SMEM_BYTES = UNIT_OFF + (QUANT ? Q_BUFS * 1024 + 128 : 0) + 1024;
   static_assert(SMEM_BYTES + 2048 <= 232448, "shared memory exceeds 227 KB");
   static constexpr int TMEM_COLS = 512;
   static constexpr int T_S = 0;
@@ -107,30 +114,67 @@ __device__ __forceinline__ bool next_part_warp(ChunkWalk& w, const PagedSeqs& s,
   return more;
 }
 
-// 16 codes times their row's scale as 16 bf16.
+// 16 codes times a factor as 16 fp16.
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 2^e, and the exponent e that brings max_code * scale into (2^14, 2^15] (0 for a scale of 0).
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int unit_exponent(uint32_t scale_bits, float max_code) {
+  if (scale_bits == 0u) return 0;
+  const int e = (int)(__float_as_uint(__uint_as_float(scale_bits) * max_code) >> 23) - 127;  // floor(log2)
+  return min(max(e - 14, -100), 100);
+}
+
 template <int FMT>
-__device__ __forceinline__ void expand16(const uint4& q, float scale, uint4 (&out)[2]) {
+__device__ __forceinline__ void expand16(const uint4& q, float factor, uint4 (&out)[2]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   uint32_t r[8];
+  const __half2 f = __float2half2_rn(factor);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float f[4];
+    uint32_t p[2];  // the codes as fp16, exactly
     if constexpr (FMT == KV_E4M3) {
+      asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+          "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+          : "=r"(p[0]), "=r"(p[1])
+          : "r"(w[i]));
+    } else {
+      // code + 128 as the low bits of 1024; then 1152 is taken off
+      const uint32_t b = w[i] ^ 0x80808080u, bias = 0x64806480u;
+      p[0] = __byte_perm(b, 0x64646464u, 0x4140);
+      p[1] = __byte_perm(b, 0x64646464u, 0x4342);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[i] >> (16 * h)) & 0xFFFFu), __NV_E4M3);
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw));
-        f[2 * h] = v.x;
-        f[2 * h + 1] = v.y;
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&p[h]), *reinterpret_cast<const __half2*>(&bias));
+        p[h] = *reinterpret_cast<const uint32_t*>(&x);
       }
-    } else {
-      // code + 128 as the low bits of 2^23, exactly; then 2^23 + 128 is taken off
-      const uint32_t b = w[i] ^ 0x80808080u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7440 + e)) - 8388736.0f;
     }
-    r[2 * i] = pack_bf16(f[0] * scale, f[1] * scale);
-    r[2 * i + 1] = pack_bf16(f[2] * scale, f[3] * scale);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&p[h]), f);
+      r[2 * i + h] = *reinterpret_cast<const uint32_t*>(&x);
+    }
   }
   out[0] = make_uint4(r[0], r[1], r[2], r[3]);
   out[1] = make_uint4(r[4], r[5], r[6], r[7]);
@@ -182,7 +226,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::Q_BUFS; ++i) {
-      mbar_init(&q_full[i], 1);
+      mbar_init(&q_full[i], C::QUANT ? 4 : 1);
       mbar_init(&q_empty[i], 1);
     }
     for (int s = 0; s < C::STAGES; ++s) {
@@ -239,7 +283,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
 
   if (warp < 4) {
     if constexpr (!C::QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_LOW));
-    if (busy && warp == 0 && lane == 0) {
+    if (!C::QUANT && busy && warp == 0 && lane == 0) {
       tma_prefetch_desc(&tm_q);
       int g = 0;
       bool ok = true;
@@ -255,7 +299,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           for (int kb = 0; kb < C::KB; ++kb)
             tma_load_3d(qbase + t * C::TILE_BYTES + kb * 16384, &tm_q, &q_full[qs], 64 * kb, w.it.kvh * p.group,
                         w.it.seq.q0 + w.it.rt * shape.tile_tokens + t * tile_tokens);
-        if constexpr (!C::QUANT) {
+        {
           const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
           const int page_size = 1 << page_log2, kvh = w.it.kvh, visible = w.visible, j1 = w.j1;
           for (int j = w.j0; j < j1; ++j, ++g) {
@@ -294,8 +338,9 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         if (!ok || !next_part(w, p.seqs, shape)) break;
       }
     } else if (busy && warp == 1 && lane == 0) {
-      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false);
-      constexpr uint32_t IDESC_O = idesc_bf16_f32(128, C::O_COLS, false, true);
+      constexpr uint32_t F16 = C::QUANT ? (1u << 7) | (1u << 10) : 0u;  // A and B format: bf16 -> fp16
+      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false) ^ F16;
+      constexpr uint32_t IDESC_O = idesc_bf16_f32(128, C::O_COLS, false, true) ^ F16;
       int g = 0;
       uint32_t zeroed_parity = 0;  // bit per stage
       int pn[2] = {0, 0}, on[2] = {0, 0};
@@ -405,12 +450,16 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
       // K and V of a tile in turn: the next one's codes are in flight while one is expanded, page ids are read
       // a tile ahead.
       const int tid = threadIdx.x - 384;
-      constexpr int PER_ROW = HD / 16;        // pieces per token
+      constexpr int PER_ROW = HD / 16;        // pieces of 16 codes per token
       constexpr int PIECES = PER_ROW;         // per thread and tile: tokens tid / PER_ROW + i * 128 / PER_ROW
       const int piece = tid % PER_ROW, tok0 = tid / PER_ROW;
+      // scales of the unit's tokens and their maxima per warp, double-buffered: one barrier of the warpgroup a unit
+      __shared__ float scales[2][2][128];
+      __shared__ uint2 maxima[2][4];
       int cell[PIECES], next_page[PIECES];    // cell: (page, head, offset) index, -1 if nothing is visible there
       uint4 q[2][PIECES];
-      float sc[2][PIECES];
+      int next_scale_page;
+      float k_scale, v_scale;                 // of token tid
       int j = busy ? w.j0 : 0;
       auto read_pages = [&]() {
 #pragma unroll
@@ -418,6 +467,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           const int t = j * 128 + tok0 + i * (128 / PER_ROW);
           next_page[i] = t < w.visible ? p.seqs.table[(long long)w.it.b * p.seqs.table_stride + (t >> page_log2)] : -1;
         }
+        const int t = j * 128 + tid;
+        next_scale_page = t < w.visible ? p.seqs.table[(long long)w.it.b * p.seqs.table_stride + (t >> page_log2)] : -1;
       };
       auto resolve = [&]() {
 #pragma unroll
@@ -433,56 +484,125 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
       };
       auto load_codes = [&](int v) {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(v ? p.pool.v : p.pool.k) + piece * 16;
-        const float* scales = v ? p.pool.v_scale : p.pool.k_scale;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int c = cell[i];
           q[v][i] = make_uint4(0u, 0u, 0u, 0u);
-          sc[v][i] = 0.f;
-          if (c >= 0) {
-            q[v][i] = *reinterpret_cast<const uint4*>(src + (long long)c * HD);
-            sc[v][i] = scales[c];
-          }
+          if (cell[i] >= 0) q[v][i] = *reinterpret_cast<const uint4*>(src + (long long)cell[i] * HD);
         }
       };
+      auto load_scales = [&]() {
+        k_scale = v_scale = 0.f;
+        if (next_scale_page >= 0 && next_scale_page < p.seqs.n_pages) {
+          const int c = ((next_scale_page * shape.kv_heads + w.it.kvh) << page_log2) +
+                        ((j * 128 + tid) & ((1 << page_log2) - 1));
+          k_scale = p.pool.k_scale[c];
+          v_scale = p.pool.v_scale[c];
+        }
+      };
+      // Q: a thread takes a row of each tile
+      auto load_q = [&](int k) {
+        const int qs = k % C::Q_BUFS;
+        const bool free = k < C::Q_BUFS || mbar_wait_bounded(&q_empty[qs], ((k / C::Q_BUFS) - 1) & 1, abort_flag,
+                                                             p.errs, kErrAttnWait, 10);
+        if (!__all_sync(0xffffffffu, free)) return false;
+        const int tok_in_tile = tid / p.group, head = tid % p.group;
+        for (int t = 0; t < w.n_tiles; ++t) {
+          const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
+          const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
+          const __nv_bfloat16* src = p.q + (long long)(w.it.seq.q0 + tok) * p.q_stride_t +
+                                     (long long)(w.it.kvh * p.group + head) * p.q_stride_h;
+          uint4 x[HD / 8];
+          uint32_t top = 0u;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            x[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
+                                         __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
+          }
+          const int e = min(max((int)(max(top & 0xFFFFu, top >> 16) >> 7), 2), 252);  // biased exponent of the maximum
+          const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+          reinterpret_cast<float*>(smem + C::UNIT_OFF)[(qs * 2 + t) * 128 + tid] = __uint_as_float((uint32_t)e << 23);
+          uint8_t* row = smem + C::Q_OFF + qs * 2 * C::TILE_BYTES + t * C::TILE_BYTES + tid * 128;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            uint4 y;
+            y.x = pack_f16(bf16lo(x[i].x) * down, bf16hi(x[i].x) * down);
+            y.y = pack_f16(bf16lo(x[i].y) * down, bf16hi(x[i].y) * down);
+            y.z = pack_f16(bf16lo(x[i].z) * down, bf16hi(x[i].z) * down);
+            y.w = pack_f16(bf16lo(x[i].w) * down, bf16hi(x[i].w) * down);
+            *reinterpret_cast<uint4*>(row + (i >> 3) * 16384 + (((i ^ tid) & 7) << 4)) = y;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[qs]);
+        return true;
+      };
+      // Once a wait has run out, `ok` stays false: nothing more is waited for or handed over, but the warps go
+      // through the rest of the range together, since they meet at a barrier for every unit.
+      bool ok = busy;
+      int k = 0;
       if (busy) {
         read_pages();
+        ok = load_q(0);
         resolve();
         load_codes(0);
+        load_scales();
       }
-      for (int g = 0; busy; ++g) {
+      bool more = busy;
+      for (int g = 0; more; ++g) {
         const int st = g % C::STAGES;
-        bool more = true;
+        bool new_item = false;
+        // the unit's powers of two
+        scales[g & 1][0][tid] = k_scale;
+        scales[g & 1][1][tid] = v_scale;
+        // scales are not negative; a NaN does not count here
+        uint32_t km = __reduce_max_sync(0xffffffffu, k_scale == k_scale ? __float_as_uint(k_scale) : 0u);
+        uint32_t vm = __reduce_max_sync(0xffffffffu, v_scale == v_scale ? __float_as_uint(v_scale) : 0u);
+        if (lane == 0) maxima[g & 1][warp & 3] = make_uint2(km, vm);
+        named_bar(1, 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          km = max(km, maxima[g & 1][i].x);
+          vm = max(vm, maxima[g & 1][i].y);
+        }
+        const int ke = unit_exponent(km, kv_code_max(FMT)), ve = unit_exponent(vm, kv_code_max(FMT));
+        const float kf = pow2i(-ke), vf = pow2i(-ve);
         if (++j == w.j1) {
-          more = next_part_warp(w, p.seqs, shape, lane);
+          more = new_item = next_part_warp(w, p.seqs, shape, lane);
           j = 0;
         }
         if (more) read_pages();
-        bool ok = true;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           if (v == 0) {
             load_codes(1);
-            ok = mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0);
+            ok = ok && mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0);
+            ok = __all_sync(0xffffffffu, ok);
+            if (tid == 0 && ok)
+              reinterpret_cast<float2*>(smem + C::UNIT_OFF + C::Q_BUFS * 1024)[st] = make_float2(pow2i(ke), (float)ve);
           } else if (more) {
             resolve();
             load_codes(0);
+            load_scales();
           }
           uint8_t* dst = smem + C::KV_OFF + st * C::STAGE_BYTES + v * C::TILE_BYTES + (piece >> 2) * 16384;
+          if (ok) {
 #pragma unroll
-          for (int i = 0; i < PIECES; ++i) {
-            const int tok = tok0 + i * (128 / PER_ROW);
-            uint4 x[2];
-            expand16<FMT>(q[v][i], sc[v][i], x);
+            for (int i = 0; i < PIECES; ++i) {
+              const int tok = tok0 + i * (128 / PER_ROW);
+              uint4 x[2];
+              expand16<FMT>(q[v][i], scales[g & 1][v][tok] * (v ? vf : kf), x);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (ok) *reinterpret_cast<uint4*>(dst + tok * 128 + ((((piece & 3) * 2 + h) ^ (tok & 7)) << 4)) = x[h];
+              for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<uint4*>(dst + tok * 128 + ((((piece & 3) * 2 + h) ^ (tok & 7)) << 4)) = x[h];
+            }
           }
         }
         fence_proxy_async_smem();
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_arrive(&kv_full[st]);
-        if (!more) break;
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&kv_full[st]);
+        if (new_item) ok = ok && load_q(++k);
       }
     }
   } else {
@@ -495,15 +615,15 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     const uint32_t o_cols = tmem + lane_off + C::T_O + t * C::O_COLS;
     const float scale2 = p.scale * kLog2e;
     const int tok_in_tile = r / p.group, head = r % p.group;
-    int sn = 0, on = 0;
+    int sn = 0, on = 0, g = 0;
     for (int part_no = 0; busy; ++part_no) {
+      const int j0 = w.j0, j1 = w.j1;
       if (t < w.n_tiles) {
         const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
         const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
         const int lim = live ? w.it.seq.len - w.it.seq.qn + tok + 1 : 0;  // tokens that this row sees
         float m_used = -INFINITY, l = 0.f;
         bool ok = true;
-        const int j0 = w.j0, j1 = w.j1;
         for (int j = j0; j < j1; ++j) {
           if (!mbar_wait_bounded(&s_full[t], sn & 1, abort_flag, p.errs, kErrAttnWait, 11 + t)) {
             ok = false;
@@ -512,6 +632,14 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           ++sn;
           tc_fence_after();
           const int seen = lim - j * 128;
+          // scores to log2 units; 8-bit: plus V's exponent
+          float to_log2 = scale2, v_exp = 0.f;
+          if constexpr (C::QUANT) {
+            const float* units = reinterpret_cast<const float*>(smem + C::UNIT_OFF);
+            const float2 u = reinterpret_cast<const float2*>(units + C::Q_BUFS * 256)[(g + j - j0) % C::STAGES];
+            to_log2 = scale2 * units[((part_no % C::Q_BUFS) * 2 + t) * 128 + r] * u.x;
+            v_exp = u.y;
+          }
           uint32_t s[C::QUANT ? 2 : 4][32];  // 8-bit: two buffers of 32 scores, else the row's 128
           float mx8[8];
           if constexpr (C::QUANT) {
@@ -544,7 +672,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                                          __uint_as_float(s[e >> 5][(e + 1) & 31]));
           }
           const float mx = fmax3f(fmax3f(mx8[0], mx8[1], mx8[2]), fmax3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-          const float m_row = mx * scale2;
+          const float m_row = C::QUANT ? fmaf(mx, to_log2, v_exp) : mx * scale2;
           if (j == j0) {
             m_used = m_row;
           } else if (__any_sync(0xffffffffu, m_row > m_used + kRescaleThreshold)) {
@@ -571,8 +699,19 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             }
             m_used = m_new;
           }
-          const float m_sub = m_used == -INFINITY ? 0.f : m_used;  // nothing seen yet: all probabilities 0
-          float rs8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          // nothing seen yet: all probabilities 0
+          const float m_sub = m_used == -INFINITY ? 0.f : m_used - (C::QUANT ? kHeadroom + v_exp : 0.f);
+          uint64_t sums[4] = {0ull, 0ull, 0ull, 0ull};  // pairs of fp32 zeros
+          const uint64_t scale_pair = pair(to_log2, to_log2), m_pair = pair(-m_sub, -m_sub);
+          // the probabilities of two columns, in their sums and packed for the product with V
+          auto weigh = [&](uint32_t s0, uint32_t s1, int e) {
+            float p0, p1;
+            unpair(fma2(pair(__uint_as_float(s0), __uint_as_float(s1)), scale_pair, m_pair), p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+            if constexpr (!C::ONES) sums[(e >> 1) & 3] = add2(sums[(e >> 1) & 3], pair(p0, p1));
+            return C::QUANT ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+          };
           if constexpr (C::QUANT) {
             tmem_ld_32x32b_x32(s_cols, s[0]);
 #pragma unroll
@@ -582,33 +721,21 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
               uint32_t pr[16];
               mask32(s[q4 & 1], seen - 32 * q4);
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float p0 = ex2_approx(fmaf(__uint_as_float(s[q4 & 1][e]), scale2, -m_sub));
-                const float p1 = ex2_approx(fmaf(__uint_as_float(s[q4 & 1][e + 1]), scale2, -m_sub));
-                if constexpr (!C::ONES) {
-                  rs8[e & 7] += p0;
-                  rs8[(e + 1) & 7] += p1;
-                }
-                pr[e >> 1] = pack_bf16(p0, p1);
-              }
+              for (int e = 0; e < 32; e += 2) pr[e >> 1] = weigh(s[q4 & 1][e], s[q4 & 1][e + 1], e);
               tmem_st_32x32b_x16(s_cols + 16 * q4, pr);  // over scores that have been read
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), scale2, -m_sub));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), scale2, -m_sub));
-              if constexpr (!C::ONES) {
-                rs8[e & 7] += p0;
-                rs8[(e + 1) & 7] += p1;
-              }
-              s[e >> 6][(e >> 1) & 31] = pack_bf16(p0, p1);
-            }
+            for (int e = 0; e < 128; e += 2)
+              s[e >> 6][(e >> 1) & 31] = weigh(s[e >> 5][e & 31], s[e >> 5][(e + 1) & 31], e);
             tmem_st_32x32b_x32(s_cols + 0, s[0]);
             tmem_st_32x32b_x32(s_cols + 32, s[1]);
           }
-          if constexpr (!C::ONES)
-            l += ((rs8[0] + rs8[1]) + (rs8[2] + rs8[3])) + ((rs8[4] + rs8[5]) + (rs8[6] + rs8[7]));
+          if constexpr (!C::ONES) {
+            float lo, hi;
+            unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), lo, hi);
+            l += C::QUANT ? (lo + hi) * ex2_approx(-v_exp) : lo + hi;
+          }
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -662,6 +789,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         }
         if (!whole && live) ws.ml[(size_t)slot * kItemRows + row] = make_float2(m_used, l);
       }
+      g += j1 - j0;
       if (!next_part_warp(w, p.seqs, shape, lane)) break;
     }
   }
