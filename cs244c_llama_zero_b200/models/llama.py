@@ -21,7 +21,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 from functools import partial
-from typing import Any, Optional, Tuple
+from typing import TYPE_CHECKING, Any, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -29,6 +29,9 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as activation_checkpoint
 
 from .config import ModelConfig
+
+if TYPE_CHECKING:
+    from .kv_cache import PagedKVCache
 
 BACKENDS = ("torch", "b200")
 
@@ -359,17 +362,105 @@ class LlamaForCausalLM(nn.Module):
             return self._zero3_executor.call_module(module_name, module, *args)
         return module(*args)
 
+    # --------------------------------------------------------------- decoding
+    @torch.no_grad()
+    def decode_step(self, input_ids: torch.Tensor, cache: "PagedKVCache", seqs: Sequence[int], rows: Sequence[int],
+                    weights: Optional[List[Any]] = None) -> torch.Tensor:
+        """Logits [len(seqs), vocab] after each sequence's last new token (B200 backend).
+
+        ``input_ids`` [sum(rows)] holds ``rows[i]`` new tokens of cached sequence ``seqs[i]``, one sequence
+        after the other: prompts, chunks of prompts or single tokens in any mixture.  Their keys and values
+        are added to ``cache``.  ``weights``: :meth:`decode_weights`, to lay them out once for many steps.
+        """
+        from ..ops import functional as B
+
+        self._check_decodable()
+        if input_ids.ndim != 1 or input_ids.numel() != sum(rows) or min(rows, default=0) < 1:
+            raise ValueError("decode_step: input_ids must be [sum(rows)] with at least one row per sequence")
+        longest = max(cache.length(s) + n for s, n in zip(seqs, rows))
+        if longest > self.cfg.max_seq_len:
+            raise ValueError(f"decode_step: {longest} tokens exceed max_seq_len {self.cfg.max_seq_len}")
+        weights = self.decode_weights() if weights is None else weights
+        batch = cache.extend(seqs, rows)
+        cos, sin = (t[:, batch.positions].contiguous() for t in B.rope_tables_t(
+            self.cfg.max_seq_len, self.cfg.head_dim, self.cfg.rope_theta, input_ids.device))
+        x = self.tok_embeddings(input_ids)
+        for w, pages in zip(weights, cache.layers):
+            x = B.decode_block(x, w, self.cfg, pages, batch, cos, sin)
+        if batch.q_starts is not None:
+            x = x[(batch.q_starts[1:] - 1).long()]
+        return self.lm_head(self.norm(x))
+
+    def decode_weights(self) -> List[Any]:
+        """Every block's weights as :meth:`decode_step` reads them (q|k|v and gate|up fused)."""
+        from ..ops import functional as B
+
+        self._check_decodable()
+        return [B.decode_weights(block) for block in self.layers]
+
+    def _check_decodable(self) -> None:
+        if self.backend != "b200":
+            raise ValueError("decoding over a key/value cache needs the b200 backend")
+        if self._zero3_executor is not None:
+            raise ValueError("decoding over a key/value cache needs the whole model on the GPU, not ZeRO-3 shards")
+
     @torch.no_grad()
     def generate(
-        self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 1.0, top_k: Optional[int] = None
+        self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 1.0, top_k: Optional[int] = None,
+        kv_cache: Optional[str] = None, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+        presence_penalty: float = 0.0, logit_bias: Optional[torch.Tensor] = None,
+        allowed_tokens: Optional[torch.Tensor] = None,
     ) -> torch.Tensor:
-        """Autoregressive sampling over a sliding ``max_seq_len`` window; ``temperature <= 0`` is greedy."""
+        """Autoregressive sampling over a sliding ``max_seq_len`` window; ``temperature <= 0`` is greedy.
+
+        On the B200 backend, ``kv_cache`` (``"bf16"``, ``"e4m3"`` or ``"int8"``) keeps keys and values in a
+        paged cache of that format, so that every token is computed once and prompts may have any length;
+        prompt and new tokens must then fit ``max_seq_len`` (a window that slides would change what the
+        cached tokens have seen).  The penalties, ``logit_bias`` (float32 ``[vocab]``) and
+        ``allowed_tokens`` (bitmask) are those of ``ops.functional.adjust_logits``.
+        """
         self.eval()
-        out = input_ids
-        for _ in range(max_new_tokens):
-            last = self(out[:, -self.cfg.max_seq_len:]).logits[:, -1]
-            out = torch.cat([out, self._pick_next(last, temperature, top_k)], dim=1)
+        batch, prompt = input_ids.shape
+        adjust = (repetition_penalty != 1.0 or frequency_penalty != 0.0 or presence_penalty != 0.0
+                  or logit_bias is not None or allowed_tokens is not None)
+        if adjust and self.backend != "b200":
+            raise ValueError("penalties, biases and token masks need the b200 backend")
+        if kv_cache is not None:
+            self._check_decodable()
+            if prompt < 1 or prompt + max_new_tokens - 1 > self.cfg.max_seq_len:
+                raise ValueError(f"generate: a prompt of {prompt} and {max_new_tokens} new tokens do not fit "
+                                 f"max_seq_len {self.cfg.max_seq_len} with a key/value cache")
+        out = torch.empty(batch, prompt + max_new_tokens, dtype=input_ids.dtype, device=input_ids.device)
+        out[:, :prompt] = input_ids
+        cache = weights = None
+        if kv_cache is not None and max_new_tokens > 0:
+            from .kv_cache import PagedKVCache
+
+            cache = PagedKVCache.for_batch(self.cfg, batch, prompt + max_new_tokens - 1, dtype=kv_cache,
+                                           device=input_ids.device)
+            weights = self.decode_weights()
+        for n in range(prompt, prompt + max_new_tokens):
+            if cache is None:
+                last = self(out[:, max(0, n - self.cfg.max_seq_len):n]).logits[:, -1]
+            else:
+                new = out[:, :n] if n == prompt else out[:, n - 1:n]
+                last = self.decode_step(new.reshape(-1), cache, range(batch), [new.shape[1]] * batch, weights)
+            if adjust:
+                last = self._adjust(last, out, n, prompt, repetition_penalty, frequency_penalty, presence_penalty,
+                                    logit_bias, allowed_tokens)
+            out[:, n:n + 1] = self._pick_next(last, temperature, top_k)
         return out
+
+    @staticmethod
+    def _adjust(logits, tokens, n, prompt, repetition, frequency, presence, bias, allowed) -> torch.Tensor:
+        from ..ops import functional as B
+
+        def per_row(value, dtype):
+            return torch.full((tokens.shape[0],), value, dtype=dtype, device=logits.device)
+
+        return B.adjust_logits(logits, tokens.long(), per_row(n, torch.int32), per_row(prompt, torch.int32),
+                               per_row(repetition, torch.float32), per_row(frequency, torch.float32),
+                               per_row(presence, torch.float32), bias, allowed)
 
     @staticmethod
     def _pick_next(logits: torch.Tensor, temperature: float, top_k: Optional[int]) -> torch.Tensor:

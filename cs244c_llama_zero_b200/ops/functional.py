@@ -578,6 +578,52 @@ def transformer_block(x: torch.Tensor, block) -> torch.Tensor:
     return _BlockFn.apply(x, *params, (block.cfg, params))
 
 
+# ------------------------------------------------------------------------------ decoding over a cache
+class DecodeWeights(NamedTuple):
+    """A block's weights as the decoding kernels read them (q|k|v and gate|up as one matrix each)."""
+
+    input_norm: torch.Tensor
+    qkv: torch.Tensor
+    o: torch.Tensor
+    post_norm: torch.Tensor
+    gate_up: torch.Tensor
+    down: torch.Tensor
+
+
+def decode_weights(block) -> DecodeWeights:
+    """Views of the block's weights where q|k|v and gate|up are adjacent in memory, else copies of those two."""
+    a, m = block.attn, block.mlp
+    return DecodeWeights(block.input_norm.weight.detach(),
+                         fused_weight([a.q_proj.weight, a.k_proj.weight, a.v_proj.weight]), a.o_proj.weight.detach(),
+                         block.post_attn_norm.weight.detach(),
+                         fused_weight([m.gate_proj.weight, m.up_proj.weight]), m.down_proj.weight.detach())
+
+
+def decode_block(x: torch.Tensor, w: DecodeWeights, cfg, pages: KVPages, batch, cos: torch.Tensor,
+                 sin: torch.Tensor) -> torch.Tensor:
+    """One transformer block for the new tokens ``x`` [tokens, dim] of ``batch`` (a ``CacheBatch``): their keys
+    and values go into the cache and they attend over it.  ``cos`` / ``sin``: RoPE tables gathered at the
+    tokens' positions, frequency-major ``[head_dim / 2, tokens]``."""
+    C = _ext()
+    T, H, KV, hd = x.shape[0], cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+    h = torch.empty_like(x)
+    C.rmsnorm_fwd(x, w.input_norm, h, None, cfg.rms_norm_eps)
+    qkv = torch.empty(T, (H + 2 * KV) * hd, dtype=x.dtype, device=x.device)
+    C.qkv_rope_fwd(h, w.qkv, qkv, cos, sin, T, hd, (H + KV) * hd)
+    heads = qkv.view(T, H + 2 * KV, hd)
+    kv_cache_write(pages, heads[:, H:H + KV], heads[:, H + KV:], batch.block_table, batch.kv_lens, batch.q_starts)
+    attn = paged_attention(heads[:, :H], pages, batch.block_table, batch.kv_lens, batch.q_starts, batch.max_q_len)
+    x2 = torch.empty_like(x)
+    C.linear_fwd(attn.view(T, H * hd), w.o, x2, x)
+    C.rmsnorm_fwd(x2, w.post_norm, h, None, cfg.rms_norm_eps)
+    act = torch.empty(T, cfg.ffn_dim, dtype=x.dtype, device=x.device)
+    gu = torch.empty(T, 2 * cfg.ffn_dim, dtype=x.dtype, device=x.device)
+    C.swiglu_fwd(h, w.gate_up, act, gu)
+    out = torch.empty_like(x)
+    C.linear_fwd(act, w.down, out, x2)
+    return out
+
+
 # ------------------------------------------------------------------------------ LM head + CE
 def shifted_targets(labels: torch.Tensor) -> torch.Tensor:
     """``targets[b, s] = labels[b, s+1]`` and ``-100`` at the last position of every row."""
