@@ -288,6 +288,44 @@ __global__ void __launch_bounds__(kDecodeThreads)
   const int row0 = BY_ROWS ? warp * 8 : 0;
   constexpr int row_step = BY_ROWS ? 8 * kDecodeWarps : 8;
   const int copy0 = BY_ROWS ? 0 : warp * C::ROWS;
+  // Q^T fragments of an item as bf16; rows that do not exist are zeros.  Asked for before the item ahead of it
+  // is joined and written, so that the two latencies overlap.
+  uint32_t qf[NT][KS][2];
+  float q_unit[NT][2];  // 8-bit: what the scores of rows 2 j and 2 j + 1 are multiplied by
+  auto load_q = [&](const PagedItem& x) {
+    const int tok0 = x.rt * shape.tile_tokens;
+    const int rows = min(shape.tile_tokens, x.seq.qn - tok0) * p.group;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = row0 + t * row_step + n;
+      const bool ok = r < rows;
+      const __nv_bfloat16* src = p.q + (long long)(x.seq.q0 + tok0 + r / p.group) * p.q_stride_t +
+                                 (long long)(x.kvh * p.group + r % p.group) * p.q_stride_h;
+      if constexpr (!QUANT) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qf[t][ks][0] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j) : 0u;
+          qf[t][ks][1] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j + 8) : 0u;
+        }
+      } else {  // product 4 g + x takes columns 64 g + 16 j + 4 x + {0, 1} and {2, 3}
+#pragma unroll
+        for (int g = 0; g < HD / 64; ++g) {
+          uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+          if (ok) {
+            w[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * j);
+            w[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * j + 8);
+          }
+          const uint32_t x8[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            qf[t][4 * g + k][0] = x8[2 * k];
+            qf[t][4 * g + k][1] = x8[2 * k + 1];
+          }
+        }
+      }
+    }
+  };
+  load_q(it);
   uint32_t slot_out = BY_ROWS ? smem_u32(smem) : ring;
   int stage = 0;
   bool first = true;
@@ -299,38 +337,13 @@ __global__ void __launch_bounds__(kDecodeThreads)
     const int rows = min(shape.tile_tokens, it.seq.qn - tok0) * p.group;
     const int base_pos = it.seq.len - it.seq.qn + tok0;  // position of the item's first row
     const int visible = item_visible(it.seq, it.rt, shape.tile_tokens);
-    // Q^T fragments; rows that do not exist are zeros
-    uint32_t qf[NT][KS][2];
-    float q_unit[NT][2];  // 8-bit: what the scores of rows 2 j and 2 j + 1 are multiplied by
+    if constexpr (QUANT) {  // to fp16, the row scaled by a power of two to a maximum in [1, 2)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int r = row0 + t * row_step + n;
-      const bool ok = r < rows;
-      const __nv_bfloat16* src = p.q + (long long)(it.seq.q0 + tok0 + r / p.group) * p.q_stride_t +
-                                 (long long)(it.kvh * p.group + r % p.group) * p.q_stride_h;
-      if constexpr (!QUANT) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          qf[t][ks][0] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j) : 0u;
-          qf[t][ks][1] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * j + 8) : 0u;
-        }
-      } else {  // product 4 g + x takes columns 64 g + 16 j + 4 x + {0, 1} and {2, 3}
+      for (int t = 0; t < NT; ++t) {
         uint32_t top = 0u;
 #pragma unroll
-        for (int g = 0; g < HD / 64; ++g) {
-          uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-          if (ok) {
-            w[0] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * j);
-            w[1] = *reinterpret_cast<const uint4*>(src + 64 * g + 16 * j + 8);
-          }
-          const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            qf[t][4 * g + k][0] = x[2 * k];
-            qf[t][4 * g + k][1] = x[2 * k + 1];
-            top = __vmaxu2(top, __vmaxu2(x[2 * k] & 0x7FFF7FFFu, x[2 * k + 1] & 0x7FFF7FFFu));
-          }
-        }
+        for (int ks = 0; ks < KS; ++ks)
+          top = __vmaxu2(top, __vmaxu2(qf[t][ks][0] & 0x7FFF7FFFu, qf[t][ks][1] & 0x7FFF7FFFu));
         uint32_t m = max(top & 0xFFFFu, top >> 16);
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -530,6 +543,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
     }
 
     // ---- join the warps
+    const int q0 = it.seq.q0 + tok0, head0 = it.kvh * p.group;
+    left -= seg;
+    if (left > 0) {
+      next_item(it, p.seqs, shape);
+      load_q(it);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -578,18 +597,16 @@ __global__ void __launch_bounds__(kDecodeThreads)
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        __nv_bfloat16* dst = p.out + (long long)(it.seq.q0 + tok0 + r / p.group) * p.o_stride_t +
-                             (long long)(it.kvh * p.group + r % p.group) * p.o_stride_h + d;
+        __nv_bfloat16* dst = p.out + (long long)(q0 + r / p.group) * p.o_stride_t +
+                             (long long)(head0 + r % p.group) * p.o_stride_h + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
       } else {
         *reinterpret_cast<float4*>(ws.o + ((size_t)slot * C::ROWS + r) * HD + d) = a;
         if (d == 0) ws.ml[(size_t)slot * C::ROWS + r] = make_float2(mx, sum);
       }
     }
-    left -= seg;
     if (left == 0) break;
     first = false;
-    next_item(it, p.seqs, shape);
     unit = 0;
     __syncthreads();  // the merge buffers are free
   }
@@ -601,18 +618,19 @@ __global__ void __launch_bounds__(kDecodeThreads)
 // the parts of a row; ROWS rows per part.  Few and large blocks: most find nothing to do, and a launch of one
 // block per row (28000 for 64 rows) took 25 us for that alone.
 constexpr int kJoinThreads = 256;
+constexpr int kAhead = 4;
 template <int HD, int ROWS, int WARPS_PER_ROW>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
   pdl_wait_and_release();
   constexpr int ROWS_AT_ONCE = kJoinThreads / 32 / WARPS_PER_ROW;
   constexpr int V = HD / 32;  // columns per lane
+  const int c = blockIdx.x + 1;
   const long long total = ws.total[0];
   const int blocks = (int)ws.total[1];
-  const int c = blockIdx.x + 1;
+  const PagedRecord rec = ws.records[c];  // there for every block, written by those with work
   if (c >= blocks) return;
   const long long u = range_begin(c, total, blocks);
-  const PagedRecord rec = ws.records[c];
   if (rec.start == u) return;                                     // no item is cut here
   if (range_begin(c - 1, total, blocks) > rec.start) return;      // cut before as well: another block's
   const int last = block_of_unit(rec.start + rec.n_units - 1, total, blocks);
@@ -629,6 +647,21 @@ __global__ void __launch_bounds__(kJoinThreads)
   for (int r0 = blockIdx.y * ROWS_AT_ONCE; r0 < rows; r0 += gridDim.y * ROWS_AT_ONCE) {
     const int r = r0 + warp / WARPS_PER_ROW;
     const bool live = r < rows;
+    // the first parts' sums are asked for together with the maxima
+    float ahead[kAhead][V];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = sub + k * WARPS_PER_ROW;
+      if (live && i < parts) {
+        const float* src = ws.o + ((size_t)slot(i) * ROWS + r) * HD + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + e);
+          ahead[k][e] = v.x;
+          ahead[k][e + 1] = v.y;
+        }
+      }
+    }
     float mx = -INFINITY;
     if (live)
       for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, ws.ml[(size_t)slot(i) * ROWS + r].x);
@@ -638,8 +671,19 @@ __global__ void __launch_bounds__(kJoinThreads)
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
     if (live) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = sub + k * WARPS_PER_ROW;
+        if (i < parts) {
+          const float2 q = ws.ml[(size_t)slot(i) * ROWS + r];
+          const float f = q.x == mx ? 1.f : ex2_approx(q.x - mx);
+          l += q.y * f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += ahead[k][e] * f;
+        }
+      }
 #pragma unroll 8
-      for (int i = sub; i < parts; i += WARPS_PER_ROW) {
+      for (int i = sub + kAhead * WARPS_PER_ROW; i < parts; i += WARPS_PER_ROW) {
         const size_t at = (size_t)slot(i) * ROWS + r;
         const float2 q = ws.ml[at];
         const float f = q.x == mx ? 1.f : ex2_approx(q.x - mx);
@@ -730,7 +774,7 @@ void launch_rows(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t
     launch_decode<FMT, HD, 2, false>(p, alloc, s);
   else if (rows <= 32)
     launch_decode<FMT, HD, 1, true>(p, alloc, s);
-  else if (rows <= 64)
+  else if (rows <= 64 && !(FMT == KV_BF16 && HD == 128))  // there two blocks fit an SM: 98 us against 62 in chunks
     launch_decode<FMT, HD, 2, true>(p, alloc, s);
   else
     paged_attention_chunk(p, alloc, s);
