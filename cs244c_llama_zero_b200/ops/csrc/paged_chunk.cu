@@ -17,6 +17,9 @@
 // scores.  V's, 2^e, goes into the exponent: the weights are 2^(s_j + e - m), with the running maximum m taken
 // over s_j + e and 2^6 of headroom, and the normaliser sums them times 2^-e.  Rounding code * scale to bf16
 // instead cost two bits of the result.
+// That is for few tiles of a sequence.  With many (a long prompt), every tile would expand the same codes again:
+// then one kernel expands all visible units once, to fp16 [sequence, unit, kv head, 128, head_dim] with their
+// powers of two beside them, and Q's rows, and the attention kernel loads both by TMA (KV_EXPANDED).
 // MMA order: S_A(0) S_B(0) | PV_A(j) S_A(j+1) PV_B(j) S_B(j+1) | ...
 //
 // Masking is by selection (a masked score becomes -inf whatever K holds), and V's rows behind the last visible
@@ -46,9 +49,22 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kHeadroom = 6.0f;          // 8-bit: log2 of the largest weight (before lazy raises)
 constexpr int kItemRows = 256;
 
+// 8-bit pages that have been expanded to fp16 units.
+constexpr int KV_EXPANDED = 3;
+struct ExpandedUnits {
+  __half* k;  // [batch, units, kv_heads, 128, head_dim]
+  __half* v;
+  float2* power;    // [batch, units, kv_heads]: 2^e of K, e of V
+  __half* q;        // [total_q, heads, head_dim]
+  float* q_power;   // [total_q, heads]
+  int units;        // of a sequence (by the block table's width)
+};
+
 template <int FMT, int HD>
 struct ChunkCfg {
-  static constexpr bool QUANT = FMT != KV_BF16;
+  static constexpr bool EXPANDED = FMT == KV_EXPANDED;
+  static constexpr bool QUANT = FMT == KV_E4M3 || FMT == KV_INT8;
+  static constexpr bool F16 = EXPANDED || QUANT;
   static constexpr int THREADS = QUANT ? 512 : 384;
   static constexpr int LAUNCH_REGS = QUANT ? 128 : 168;
   static constexpr int KB = HD / 64;
@@ -56,14 +72,14 @@ struct ChunkCfg {
   static constexpr int STAGES = (HD == 64) ? 3 : 2;
   static constexpr int Q_BUFS = (HD == 64) ? 2 : 1;
   // bf16: a softmax thread keeps its row's 128 scores in registers, for which the first warpgroup hands over
-  // some of its own.  8-bit: the expanding warpgroup leaves 128 registers per thread, and the scores are read
-  // from tensor memory twice, 32 at a time (holding them spilled, and a unit took 7 us instead of SOON).
+  // some of its own.  8-bit expanded here: the fourth warpgroup leaves 128 registers per thread, and the scores are
+  // read from tensor memory twice, 32 at a time (holding them spilled: 7.2 us a unit instead of 4.7 at head_dim 128).
   static constexpr int REGS_LOW = 88;
   static constexpr int REGS_HIGH = 208;
   static constexpr int REGS_NEEDED = QUANT ? 0 : 128 * REGS_LOW + 256 * REGS_HIGH;
   static_assert(REGS_NEEDED <= THREADS * LAUNCH_REGS, "register split over budget");
   // hd 64: row sums from the tensor cores, by a block of ones behind V (see the training forward kernel)
-  static constexpr bool ONES = (HD == 64) && !QUANT;  // (8-bit: the sums are weighted for each unit)
+  static constexpr bool ONES = (HD == 64) && !F16;  // (8-bit: the sums are weighted for each unit)
   static constexpr int O_COLS = ONES ? HD + 16 : HD;
   static constexpr int STAGE_BYTES = (ONES ? 3 : 2) * TILE_BYTES;
   static constexpr int Q_OFF = 0;
@@ -205,7 +221,7 @@ template <int FMT, int HD>
 __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnParams p,
-                       PagedShape shape, PagedWorkspace ws) {
+                       PagedShape shape, PagedWorkspace ws, ExpandedUnits ex) {
   using C = ChunkCfg<FMT, HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
@@ -310,6 +326,16 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             }
             uint8_t* ks = smem + C::KV_OFF + st * C::STAGE_BYTES;
             uint8_t* vs = ks + C::TILE_BYTES;
+            if constexpr (C::EXPANDED) {
+              const int row = ((w.it.b * ex.units + j) * shape.kv_heads + kvh) * 128;
+              mbar_expect_tx(&kv_full[st], 2 * C::TILE_BYTES);
+#pragma unroll
+              for (int kb = 0; kb < C::KB; ++kb) {
+                tma_load_2d(ks + kb * 16384, &tm_k, &kv_full[st], 64 * kb, row);
+                tma_load_2d(vs + kb * 16384, &tm_v, &kv_full[st], 64 * kb, row);
+              }
+              continue;
+            }
             const int n_pages = min(128 >> page_log2, max(0, (visible - j * 128 + page_size - 1) >> page_log2));
             // a tile that the sequence ends in gets V on a barrier of its own: warp 2 zeroes its tail first
             const bool tail = (j + 1) * 128 > visible;
@@ -338,7 +364,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         if (!ok || !next_part(w, p.seqs, shape)) break;
       }
     } else if (busy && warp == 1 && lane == 0) {
-      constexpr uint32_t F16 = C::QUANT ? (1u << 7) | (1u << 10) : 0u;  // A and B format: bf16 -> fp16
+      constexpr uint32_t F16 = C::F16 ? (1u << 7) | (1u << 10) : 0u;  // A and B format: bf16 -> fp16
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false) ^ F16;
       constexpr uint32_t IDESC_O = idesc_bf16_f32(128, C::O_COLS, false, true) ^ F16;
       int g = 0;
@@ -367,7 +393,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         for (int j = 0; ok && j < n; ++j) {
           st = (g + j) % C::STAGES;
           const int st1 = (g + j + 1) % C::STAGES;
-          if constexpr (!C::QUANT) {
+          if constexpr (!C::F16) {
             if ((j0 + j + 1) * 128 > visible) {
               if (!mbar_wait_bounded(&v_zeroed[st], (zeroed_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 7)) {
                 ok = false;
@@ -420,7 +446,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         tc_commit(&q_empty[qs]);
         if (!ok || !next_part(w, p.seqs, shape)) break;
       }
-    } else if (!C::QUANT && busy && warp == 2) {
+    } else if (!C::F16 && busy && warp == 2) {
       int g = 0;
       uint32_t raw_parity = 0;  // bit per stage
       while (true) {
@@ -623,6 +649,14 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
         const int lim = live ? w.it.seq.len - w.it.seq.qn + tok + 1 : 0;  // tokens that this row sees
         float m_used = -INFINITY, l = 0.f;
+        float q_power = 1.f;
+        float2 power = make_float2(1.f, 0.f);
+        const float2* powers = nullptr;
+        if constexpr (C::EXPANDED) {
+          powers = ex.power + (long long)w.it.b * ex.units * shape.kv_heads + w.it.kvh;
+          power = powers[(long long)j0 * shape.kv_heads];
+          if (live) q_power = ex.q_power[(long long)(w.it.seq.q0 + tok) * p.heads + w.it.kvh * p.group + head];
+        }
         bool ok = true;
         for (int j = j0; j < j1; ++j) {
           if (!mbar_wait_bounded(&s_full[t], sn & 1, abort_flag, p.errs, kErrAttnWait, 11 + t)) {
@@ -634,6 +668,11 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           const int seen = lim - j * 128;
           // scores to log2 units; 8-bit: plus V's exponent
           float to_log2 = scale2, v_exp = 0.f;
+          if constexpr (C::EXPANDED) {
+            to_log2 = scale2 * q_power * power.x;
+            v_exp = power.y;
+            if (j + 1 < j1) power = powers[(long long)(j + 1) * shape.kv_heads];  // for the next unit
+          }
           if constexpr (C::QUANT) {
             const float* units = reinterpret_cast<const float*>(smem + C::UNIT_OFF);
             const float2 u = reinterpret_cast<const float2*>(units + C::Q_BUFS * 256)[(g + j - j0) % C::STAGES];
@@ -672,7 +711,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                                          __uint_as_float(s[e >> 5][(e + 1) & 31]));
           }
           const float mx = fmax3f(fmax3f(mx8[0], mx8[1], mx8[2]), fmax3f(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-          const float m_row = C::QUANT ? fmaf(mx, to_log2, v_exp) : mx * scale2;
+          const float m_row = C::F16 ? fmaf(mx, to_log2, v_exp) : mx * scale2;
           if (j == j0) {
             m_used = m_row;
           } else if (__any_sync(0xffffffffu, m_row > m_used + kRescaleThreshold)) {
@@ -700,7 +739,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             m_used = m_new;
           }
           // nothing seen yet: all probabilities 0
-          const float m_sub = m_used == -INFINITY ? 0.f : m_used - (C::QUANT ? kHeadroom + v_exp : 0.f);
+          const float m_sub = m_used == -INFINITY ? 0.f : m_used - (C::F16 ? kHeadroom + v_exp : 0.f);
           uint64_t sums[4] = {0ull, 0ull, 0ull, 0ull};  // pairs of fp32 zeros
           const uint64_t scale_pair = pair(to_log2, to_log2), m_pair = pair(-m_sub, -m_sub);
           // the probabilities of two columns, in their sums and packed for the product with V
@@ -710,7 +749,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             p0 = ex2_approx(p0);
             p1 = ex2_approx(p1);
             if constexpr (!C::ONES) sums[(e >> 1) & 3] = add2(sums[(e >> 1) & 3], pair(p0, p1));
-            return C::QUANT ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+            return C::F16 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
           };
           if constexpr (C::QUANT) {
             tmem_ld_32x32b_x32(s_cols, s[0]);
@@ -734,7 +773,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           if constexpr (!C::ONES) {
             float lo, hi;
             unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), lo, hi);
-            l += C::QUANT ? (lo + hi) * ex2_approx(-v_exp) : lo + hi;
+            l += C::F16 ? (lo + hi) * ex2_approx(-v_exp) : lo + hi;
           }
           tc_wait_st();
           tc_fence_before();
@@ -862,8 +901,97 @@ __global__ void __launch_bounds__(kItemRows)
   }
 }
 
+// Blocks below `unit_blocks` expand one unit of one kv head each, the others a run of Q's rows.  Reads each
+// code once and writes it as fp16; bound by memory.
 template <int FMT, int HD>
-void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
+__global__ void __launch_bounds__(128) paged_expand_kernel(PagedAttnParams p, ExpandedUnits ex, int unit_blocks) {
+  pdl_wait_and_release();
+  constexpr int LANES = HD / 8;  // per row of Q
+  const int tid = threadIdx.x, lane = tid & 31;
+  if ((int)blockIdx.x >= unit_blocks) {
+    const long long row = (long long)((int)blockIdx.x - unit_blocks) * (128 / LANES) + tid / LANES;
+    const int sub = tid % LANES;
+    if (row >= (long long)p.seqs.total_q * p.heads) return;  // whole groups of LANES lanes
+    const __nv_bfloat16* src = p.q + row / p.heads * p.q_stride_t + row % p.heads * p.q_stride_h + sub * 8;
+    const uint4 x = *reinterpret_cast<const uint4*>(src);
+    const uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu),
+                                  __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+    uint32_t m = max(top & 0xFFFFu, top >> 16);
+    const uint32_t group = LANES == 32 ? 0xFFFFFFFFu : ((1u << LANES) - 1u) << (lane / LANES * LANES);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(group, m, o));
+    const int e = min(max((int)(m >> 7), 2), 252);  // biased exponent of the row's maximum
+    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+    uint4 y;
+    y.x = pack_f16(bf16lo(x.x) * down, bf16hi(x.x) * down);
+    y.y = pack_f16(bf16lo(x.y) * down, bf16hi(x.y) * down);
+    y.z = pack_f16(bf16lo(x.z) * down, bf16hi(x.z) * down);
+    y.w = pack_f16(bf16lo(x.w) * down, bf16hi(x.w) * down);
+    *reinterpret_cast<uint4*>(ex.q + row * HD + sub * 8) = y;
+    if (sub == 0) ex.q_power[row] = __uint_as_float((uint32_t)e << 23);
+    return;
+  }
+  const int kvh = (int)blockIdx.x % p.pool.kv_heads, u = (int)blockIdx.x / p.pool.kv_heads;
+  const int b = u / ex.units, j = u % ex.units;
+  const SeqInfo seq = seq_info(p.seqs, b);
+  if (seq.qn == 0 || j * 128 >= max(seq.len, 1)) return;  // (an empty sequence still has one unit, of zeros)
+  __shared__ float scales[2][128];
+  __shared__ int cells[128];
+  __shared__ uint2 maxima[4];
+  int cell = -1;
+  const int t = j * 128 + tid;
+  if (t < seq.len) {
+    const int page = p.seqs.table[(long long)b * p.seqs.table_stride + (t >> p.seqs.page_log2)];
+    if (page >= 0 && page < p.seqs.n_pages)
+      cell = ((page * p.pool.kv_heads + kvh) << p.seqs.page_log2) + (t & ((1 << p.seqs.page_log2) - 1));
+    else
+      report_error(p.errs, kErrBadIndex, b);
+  }
+  const float ks = cell >= 0 ? p.pool.k_scale[cell] : 0.f, vs = cell >= 0 ? p.pool.v_scale[cell] : 0.f;
+  cells[tid] = cell;
+  scales[0][tid] = ks;
+  scales[1][tid] = vs;
+  // scales are not negative; a NaN does not count here
+  uint32_t km = __reduce_max_sync(0xffffffffu, ks == ks ? __float_as_uint(ks) : 0u);
+  uint32_t vm = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
+  if (lane == 0) maxima[tid >> 5] = make_uint2(km, vm);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    km = max(km, maxima[i].x);
+    vm = max(vm, maxima[i].y);
+  }
+  const int ke = unit_exponent(km, kv_code_max(FMT)), ve = unit_exponent(vm, kv_code_max(FMT));
+  const float kf = pow2i(-ke), vf = pow2i(-ve);
+  if (tid == 0) ex.power[blockIdx.x] = make_float2(pow2i(ke), (float)ve);
+  constexpr int PER_ROW = HD / 16;
+  const int piece = tid % PER_ROW;
+#pragma unroll
+  for (int i = 0; i < PER_ROW; ++i) {
+    const int tok = tid / PER_ROW + i * (128 / PER_ROW);
+    const int c = cells[tok];
+    uint4 q[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (c >= 0) {
+      q[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.pool.k) + (long long)c * HD + piece * 16);
+      q[1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.pool.v) + (long long)c * HD + piece * 16);
+    }
+    const size_t at = ((size_t)blockIdx.x * 128 + tok) * HD + piece * 16;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      uint4 x[2];
+      // nothing there: zeros, and not the NaN that 0 * a NaN code would give
+      expand16<FMT>(q[v], scales[v][tok] * (v ? vf : kf), x);
+      uint4* dst = reinterpret_cast<uint4*>((v ? ex.v : ex.k) + at);
+      dst[0] = x[0];
+      dst[1] = x[1];
+    }
+  }
+}
+
+template <int FMT, int HD>
+void launch_attention(const PagedAttnParams& p, const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                      const CUtensorMap& tm_v, const PagedShape& shape, const PagedWorkspace& ws,
+                      const ExpandedUnits& ex, cudaStream_t s) {
   using C = ChunkCfg<FMT, HD>;
   auto* kernel = paged_chunk_kernel<FMT, HD>;
   static std::atomic<unsigned long long> configured{0};
@@ -875,21 +1003,66 @@ void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_
     B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
   });
   const int blocks = num_sms_cached();
-  const PagedWorkspace ws = paged_workspace(alloc(paged_workspace_bytes(blocks, kItemRows, HD)), blocks, kItemRows);
-  const int tile_tokens = 128 / p.group;
-  const PagedShape shape{2 * tile_tokens, 7, p.pool.kv_heads};
-  const CUtensorMap tm_q = make_tmap_bf16_3d(p.q, HD, p.heads, p.seqs.total_q, p.q_stride_h, p.q_stride_t, 64,
-                                             p.group, tile_tokens);
-  CUtensorMap tm_k = tm_q, tm_v = tm_q;  // 8-bit pages are not read by TMA
-  if constexpr (!C::QUANT) {
-    const uint64_t rows = (uint64_t)p.seqs.n_pages * p.pool.kv_heads << p.seqs.page_log2;
-    tm_k = make_tmap_bf16_2d(p.pool.k, HD, rows, HD, 64, 1u << p.seqs.page_log2);
-    tm_v = make_tmap_bf16_2d(p.pool.v, HD, rows, HD, 64, 1u << p.seqs.page_log2);
-  }
-  launch_k(kernel, dim3(blocks), dim3(C::THREADS), C::SMEM_BYTES, s, 1, tm_q, tm_k, tm_v, p, shape, ws);
+  launch_k(kernel, dim3(blocks), dim3(C::THREADS), C::SMEM_BYTES, s, 1, tm_q, tm_k, tm_v, p, shape, ws, ex);
   launch_k(paged_chunk_join_kernel<HD>, dim3(blocks - 1, HD / 16), dim3(kItemRows), 0, s, 1, p, shape, ws);
   B200_CUDA_CHECK(cudaGetLastError());
   count_launch(2);
+}
+
+// Expanding once pays when rows per kv head and sequence x head_dim reach this (8 int8 caches of 8192 tokens with
+// 8 kv heads, expanded in each tile against once: head_dim 64, 256 rows 73 / 79 us, 512 rows 125 / 117;
+// head_dim 128, 128 rows 104 / 110, 256 rows 151 / 126, 512 rows 250 / 177; 8192 rows over one e4m3 cache of 16384
+// tokens 987 / 560), as long as the units by the block table's width fit this much scratch memory.
+constexpr long long kExpandRowColumns = 32768;
+constexpr size_t kExpandBytes = 512u << 20;
+
+template <int FMT, int HD>
+void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
+  const int blocks = num_sms_cached();
+  const int tile_tokens = 128 / p.group;
+  const PagedShape shape{2 * tile_tokens, 7, p.pool.kv_heads};
+  const size_t ws_bytes = (paged_workspace_bytes(blocks, kItemRows, HD) + 255) / 256 * 256;
+  auto q_map = [&](const void* q, long long stride_h, long long stride_t) {
+    return make_tmap_bf16_3d(q, HD, p.heads, p.seqs.total_q, stride_h, stride_t, 64, p.group, tile_tokens);
+  };
+  ExpandedUnits ex{};
+  if constexpr (FMT == KV_BF16) {
+    const PagedWorkspace ws = paged_workspace(alloc(ws_bytes), blocks, kItemRows);
+    const uint64_t rows = (uint64_t)p.seqs.n_pages * p.pool.kv_heads << p.seqs.page_log2;
+    launch_attention<FMT, HD>(p, q_map(p.q, p.q_stride_h, p.q_stride_t),
+                              make_tmap_bf16_2d(p.pool.k, HD, rows, HD, 64, 1u << p.seqs.page_log2),
+                              make_tmap_bf16_2d(p.pool.v, HD, rows, HD, 64, 1u << p.seqs.page_log2), shape, ws, ex, s);
+  } else {
+    ex.units = (int)((((long long)p.seqs.max_pages << p.seqs.page_log2) + 127) / 128);
+    const long long unit_blocks = (long long)p.seqs.batch * ex.units * p.pool.kv_heads;
+    const size_t kv_bytes = (size_t)unit_blocks * 128 * HD * 2;
+    const long long q_rows = (long long)p.seqs.total_q * p.heads;
+    const size_t q_bytes = (size_t)q_rows * HD * 2;
+    if ((long long)p.seqs.max_q * p.group * HD >= kExpandRowColumns && unit_blocks > 0 && 2 * kv_bytes <= kExpandBytes) {
+      const size_t power_bytes = ((size_t)unit_blocks * 8 + 255) / 256 * 256;
+      uint8_t* base = reinterpret_cast<uint8_t*>(
+          alloc(ws_bytes + 2 * kv_bytes + power_bytes + (q_bytes + 255) / 256 * 256 + (size_t)q_rows * 4));
+      const PagedWorkspace ws = paged_workspace(base, blocks, kItemRows);
+      ex.k = reinterpret_cast<__half*>(base + ws_bytes);
+      ex.v = ex.k + kv_bytes / 2;
+      ex.power = reinterpret_cast<float2*>(base + ws_bytes + 2 * kv_bytes);
+      ex.q = reinterpret_cast<__half*>(base + ws_bytes + 2 * kv_bytes + power_bytes);
+      ex.q_power = reinterpret_cast<float*>(base + ws_bytes + 2 * kv_bytes + power_bytes + (q_bytes + 255) / 256 * 256);
+      const long long q_blocks = (q_rows + 128 / (HD / 8) - 1) / (128 / (HD / 8));
+      launch_k(paged_expand_kernel<FMT, HD>, dim3((unsigned)(unit_blocks + q_blocks)), dim3(128), 0, s, 1, p, ex,
+               (int)unit_blocks);
+      count_launch(1);
+      const uint64_t rows = (uint64_t)unit_blocks * 128;
+      // (fp16 moves like bf16: the maps only copy)
+      launch_attention<KV_EXPANDED, HD>(p, q_map(ex.q, HD, (long long)p.heads * HD),
+                                        make_tmap_bf16_2d(ex.k, HD, rows, HD, 64, 128),
+                                        make_tmap_bf16_2d(ex.v, HD, rows, HD, 64, 128), shape, ws, ex, s);
+    } else {
+      const PagedWorkspace ws = paged_workspace(alloc(ws_bytes), blocks, kItemRows);
+      const CUtensorMap none = q_map(p.q, p.q_stride_h, p.q_stride_t);  // nothing is read by TMA
+      launch_attention<FMT, HD>(p, none, none, none, shape, ws, ex, s);
+    }
+  }
 }
 
 }  // namespace

@@ -105,6 +105,24 @@ def test_items_that_span_blocks(F, fmt, hd):
         _check(_attend(F, b), want, tolerance(want, mag, size, fmt != "bf16"))
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("heads", [(12, 3, 64), (8, 2, 128)])
+def test_long_chunks_of_8_bit_pages(F, fmt, heads):
+    """Enough rows that the codes are expanded once for all of a sequence's tiles; short and empty sequences,
+    rows behind the last one and a wide block table in the same batch; scales of very different size."""
+    b = Batch([520, 0, 3, 300, 5], [700, 90, 3, 300, 0], *heads, fmt, 16, seed=17, behind=3)
+    for which in range(2):  # every seventh token 2^12 times larger or smaller than the others
+        b.scales[which][:, :, ::7] *= 2.0 ** (12 if which else -12)
+    want, mag, size = b.attention()
+    wide = torch.cat([b.table, torch.full((5, 40), b.n_pages + 9, dtype=torch.int32)], 1).cuda()
+    out = torch.full(b.q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    F.paged_attention(b.q.cuda(), b.pages("cuda"), wide, b.lens.cuda(), b.starts.cuda(), b.max_q, out=out)
+    _check(out[:b.total], want, tolerance(want, mag, size, True))
+    assert (out[b.total:] == 7).all() and (out[b.total - 5:b.total] == 0).all()
+    again = F.paged_attention(b.q.cuda(), b.pages("cuda"), wide, b.lens.cuda(), b.starts.cuda(), b.max_q)
+    assert torch.equal(again[:b.total], out[:b.total])
+
+
 @pytest.mark.parametrize("fmt", list(FORMATS))
 def test_rows_before_the_first_token_are_zero(F, fmt):
     """More new tokens than cached ones: the first rows stand before the sequence and see nothing."""
