@@ -67,7 +67,7 @@ b200::KvPool check_pool(const Tensor& k, const Tensor& v, const std::optional<Te
               "tensors of one shape, got ", shape(k), " and ", shape(v));
   TORCH_CHECK(k.scalar_type() == v.scalar_type(), "k and v pages must have the same dtype");
   TORCH_CHECK(k.is_contiguous() && v.is_contiguous(), "pages must be contiguous");
-  TORCH_CHECK(k.size(1) >= 1, "pages need at least one kv head");
+  TORCH_CHECK(k.size(0) >= 1 && k.size(1) >= 1, "pages need at least one page and one kv head");
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, "head_dim must be 64 or 128, got ", std::to_string(k.size(3)));
   log2_page(k.size(2));
   TORCH_CHECK(k.size(0) * k.size(1) * k.size(2) <= INT_MAX, "the pool holds more than 2^31 - 1 rows");

@@ -31,9 +31,19 @@ DeviceErrors* device_errors_ptr() {
   std::lock_guard<std::mutex> lock(mu);
   if ((int)per_device.size() <= dev) per_device.resize(dev + 1, nullptr);
   if (per_device[dev] == nullptr) {
+    // The first kernel on a device may be one that a stream capture records: the allocation is none of the
+    // capture's business, so this thread takes it out of the capture's checks.
     DeviceErrors* p = nullptr;
-    B200_CUDA_CHECK(cudaMalloc(&p, sizeof(DeviceErrors)));
-    B200_CUDA_CHECK(cudaMemset(p, 0, sizeof(DeviceErrors)));
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    B200_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaError_t e = cudaMalloc(&p, sizeof(DeviceErrors));
+    cudaStream_t s = nullptr;
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(DeviceErrors), s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (s != nullptr) cudaStreamDestroy(s);
+    B200_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    B200_CUDA_CHECK(e);
     per_device[dev] = p;
   }
   return per_device[dev];

@@ -44,6 +44,8 @@ def test_cpu_tensors_are_refused_last(F):
     (dict(k_scale=lambda p: p.k_scale.double()), "contiguous float32"),
     (dict(v_scale=lambda p: p.v_scale[:, :1]), "contiguous float32"),
     (dict(k=lambda p: p.k[:, :, :12].contiguous(), v=lambda p: p.v[:, :, :12].contiguous()), "page_size must be"),
+    (dict(k=lambda p: p.k[:0], v=lambda p: p.v[:0], k_scale=lambda p: p.k_scale[:0], v_scale=lambda p: p.v_scale[:0]),
+     "at least one page"),
     (dict(k=lambda p: p.k[..., :32].contiguous(), v=lambda p: p.v[..., :32].contiguous()), "head_dim must be 64 or 128"),
     (dict(v=lambda p: p.v.transpose(0, 1).contiguous().transpose(0, 1)), "contiguous"),
 ])

@@ -253,6 +253,92 @@ def test_attention_repeats_bit_for_bit(F):
         assert torch.equal(_attend(F, b), first)
 
 
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("q_lens", [[1, 1], [70, 150], [520, 9]])
+def test_head_major_queries(F, fmt, q_lens):
+    """q as [heads, tokens, head_dim] in memory: the token stride is the smaller one."""
+    b = Batch(q_lens, [n + 20 for n in q_lens], 8, 2, 128, fmt, 32, seed=18)
+    table, lens, starts = _meta(b)
+    q = b.q.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+    got = F.paged_attention(q, b.pages("cuda"), table, lens, starts, b.max_q)
+    assert torch.equal(got, _attend(F, b))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "bf16"])
+@pytest.mark.parametrize("q_len", [1, 12, 60, 600])
+def test_poisoned_rows_show(F, fmt, q_len):
+    """A key or value with a NaN or an infinity, written into the cache: the rows that see it are NaN, and
+    other sequences are as before."""
+    b = Batch([q_len, q_len], [q_len + 200, q_len + 130], 4, 1, 64, fmt, 16, seed=19)
+    clean = _attend(F, b)
+    for bad_k, bad_v in ((float("nan"), None), (None, float("nan")), (None, float("inf"))):
+        pages = b.pages("cuda")
+        k, v = torch.ones(1, 1, 64, dtype=torch.bfloat16), torch.ones(1, 1, 64, dtype=torch.bfloat16)
+        if bad_k is not None:
+            k[0, 0, 3] = bad_k
+        if bad_v is not None:
+            v[0, 0, 3] = bad_v
+        at = torch.tensor([61], dtype=torch.int32).cuda()  # token 60 of sequence 0
+        F.kv_cache_write(pages, k.cuda(), v.cuda(), b.table[:1].cuda(), at)
+        out = F.paged_attention(b.q.cuda(), pages, *_meta(b), b.max_q)
+        assert torch.equal(out[q_len:], clean[q_len:])
+        if fmt == "bf16" and bad_v is not None:  # unquantised, only its column is lost
+            assert not torch.isfinite(out[:q_len, :, 3]).any()
+        else:
+            assert torch.isnan(out[:q_len]).all()
+
+
+@pytest.mark.parametrize("fmt,n_pages", [("bf16", 17000), ("int8", 34000)])
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_pools_past_32_bit_offsets(F, fmt, n_pages, q_len):
+    """Pools of more than 4 GB: the same pages at their end give the same result, and take writes there."""
+    b = Batch([q_len], [q_len + 300], 8, 8, 128, fmt, 128, seed=20)
+    small = b.pages("cuda")
+    table, lens, starts = _meta(b)
+    want = F.paged_attention(b.q.cuda(), small, table, lens, starts, b.max_q)
+    big = [None if t is None else torch.empty((n_pages,) + tuple(t.shape[1:]), dtype=t.dtype, device="cuda")
+           for t in small]
+    for s, t in zip(small, big):
+        if s is not None:
+            t[-b.n_pages:].copy_(s)
+    assert big[0].numel() * big[0].element_size() > 1 << 32
+    pages = F.KVPages(*big)
+    moved = table + (n_pages - b.n_pages)
+    assert torch.equal(F.paged_attention(b.q.cuda(), pages, moved, lens, starts, b.max_q), want)
+    F.kv_cache_write(pages, b.k.cuda(), b.v.cuda(), moved, lens, starts)
+    F.kv_cache_write(small, b.k.cuda(), b.v.cuda(), table, lens, starts)
+    for x, y in zip(F.kv_cache_read(pages, moved, lens, starts, total=q_len),
+                    F.kv_cache_read(small, table, lens, starts, total=q_len)):
+        assert torch.equal(x, y)
+
+
+def test_first_call_inside_a_capture():
+    """The process's first kernel may be one that a graph capture records."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from cs244c_llama_zero_b200.ops import functional as F
+pages = F.KVPages(*[torch.ones(4, 2, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)])
+q = torch.ones(1, 4, 64, dtype=torch.bfloat16, device="cuda")
+table = torch.tensor([[2, 1]], dtype=torch.int32).cuda()
+lens = torch.tensor([20], dtype=torch.int32).cuda()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = F.paged_attention(q, pages, table, lens)
+graph.replay()
+torch.cuda.synchronize()
+assert (out == 1).all()
+print("captured")
+"""
+    root = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------------ cache
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads", [(4, 2, 64), (8, 1, 128), (3, 3, 64)])
