@@ -5,9 +5,10 @@
 // zero get scale 0 and zero codes; rows with an infinity or a NaN get scale NaN and zero codes, so that
 // they read back as NaN instead of as some finite value.
 //
-// The quotient is formed from n = x M (exact: 8 x 9 bits) as q0 = n r, r = 1/a, followed by one exact
-// remainder step q = q0 + r (n - q0 a), which returns the correctly rounded quotient: bf16 inputs that fall
-// exactly between two codes do so in fp32 too, and no other quotient comes closer than 2^-17 to a tie.
+// The quotient is formed from n = x M (exact: 8 x 9 bits) as q0 = n r, r ~ 1/a, followed by one exact
+// remainder step q = q0 + r (n - q0 a), whose error is below 2^-20 of q0's last bit: bf16 inputs that fall
+// exactly between two codes come out exactly so, and no other quotient is closer than 2^-17 to a tie.  The scale
+// a / M is rounded correctly in the same way.
 //
 // A warp takes K or V of a run of tokens.  Where the tokens lie is found by its lanes at once, one token each
 // (a search over q_starts, the sequence's length, its page), and handed round; then 32 lanes x 16 bytes per
@@ -95,8 +96,11 @@ __global__ void __launch_bounds__(kThreads)
   float* scales = run.is_v ? pool.v_scale : pool.k_scale;
   constexpr int HEADS = 32 / LANES;  // per access
   const int passes = (pool.kv_heads + HEADS - 1) / HEADS;
-  int tok = 0, pass = 0;
   const int total = run.count * passes;
+  // source of this lane's piece of the access, advanced from access to access
+  const __nv_bfloat16* from = src + run.t0 * stride_t + (lane / LANES) * stride_h + sub * 8;
+  const long long next_pass = HEADS * stride_h, next_token = stride_t - passes * next_pass;
+  int tok = 0, pass = 0;
   for (int i0 = 0; i0 < total; i0 += kInFlight) {
     uint4 x[kInFlight];
     long long cell[kInFlight];
@@ -107,10 +111,11 @@ __global__ void __launch_bounds__(kThreads)
       const int h = pass * HEADS + lane / LANES;
       cell[i] = -1;
       if (i0 + i < total && place >= 0 && h < pool.kv_heads) {
-        cell[i] = place + ((long long)h << seqs.page_log2);
-        x[i] = *reinterpret_cast<const uint4*>(src + (run.t0 + tok) * stride_t + h * stride_h + sub * 8);
+        cell[i] = place + (h << seqs.page_log2);
+        x[i] = *reinterpret_cast<const uint4*>(from);
       }
-      if (++pass == passes) pass = 0, ++tok;
+      from += next_pass;
+      if (++pass == passes) pass = 0, ++tok, from += next_token;
     }
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
@@ -128,7 +133,7 @@ __global__ void __launch_bounds__(kThreads)
         // a power of two that brings a near 1, so that neither n nor r leaves the normal range
         const float unit = __uint_as_float((uint32_t)min(max(254 - (int)(m >> 7), 1), 240) << 23);
         const float au = a * unit, um = unit * kv_code_max(FMT);
-        const float r = m > 0u ? __frcp_rn(au) : 0.0f;
+        const float r = m > 0u ? __fdividef(1.0f, au) : 0.0f;
         float f[8];
         unpack8(x[i], f);
 #pragma unroll
@@ -155,7 +160,11 @@ __global__ void __launch_bounds__(kThreads)
         }
         if (cell[i] >= 0) {
           *reinterpret_cast<uint2*>(dst + cell[i] * HD + sub * 8) = make_uint2(w[0], w[1]);
-          if (sub == 0) scales[cell[i]] = finite ? a / kv_code_max(FMT) : __int_as_float(0x7FC00000);
+          if (sub == 0) {
+            constexpr float M = kv_code_max(FMT), inv = 1.0f / M;
+            const float s0 = a * inv;
+            scales[cell[i]] = finite ? fmaf(fmaf(-s0, M, a), inv, s0) : __int_as_float(0x7FC00000);
+          }
         }
       }
     }

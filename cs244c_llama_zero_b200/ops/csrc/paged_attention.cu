@@ -45,6 +45,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.0f;  // log2 units
+// The running maximum of a row that has seen nothing: finite, so that differences with it are numbers, and below
+// every score.
+constexpr float kNothing = -3.0e38f;
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr int kUnitLog2 = 6;  // 16 tokens per warp
@@ -367,9 +370,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][t][e] = 0.f;
-    float m[NT][2], l[NT][2];
+    float m_sub[NT][2], l[NT][2];  // the maximum in use less the headroom
 #pragma unroll
-    for (int t = 0; t < NT; ++t) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+    for (int t = 0; t < NT; ++t) m_sub[t][0] = m_sub[t][1] = kNothing, l[t][0] = l[t][1] = 0.f;
 
     // 16 tokens from t0 on, at `tile` in shared memory, against the first N row tiles
     auto step = [&](auto n_tiles, uint32_t tile, int t0) {
@@ -435,11 +438,15 @@ __global__ void __launch_bounds__(kDecodeThreads)
             if (t0 + n + 8 >= lim) s[t][2 + e] = -INFINITY;
           }
       }
-      bool raise = false;
+      // weights: 2^d with d = score - m + headroom
+      float d[N][4], top = kNothing;
 #pragma unroll
-      for (int t = 0; t < N; ++t)
-        raise |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise || fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
-      if (__any_sync(0xffffffffu, raise)) {
+      for (int t = 0; t < N; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[t][e] = s[t][e] - m_sub[t][e & 1];
+        top = fmax3f(fmax3f(top, d[t][0], d[t][1]), d[t][2], d[t][3]);
+      }
+      if (__any_sync(0xffffffffu, top > kRaise + C::HEADROOM)) {
 #pragma unroll
         for (int t = 0; t < N; ++t)
 #pragma unroll
@@ -448,25 +455,24 @@ __global__ void __launch_bounds__(kDecodeThreads)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(m[t][e], mx);
-            const float alpha = m_new == m[t][e] ? 1.f : ex2_approx(m[t][e] - m_new);
-            m[t][e] = m_new;
+            const float m_new = fmaxf(m_sub[t][e], mx - C::HEADROOM);
+            const float alpha = ex2_approx(m_sub[t][e] - m_new);
+            m_sub[t][e] = m_new;
             l[t][e] *= alpha;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
               o[i][t][e] *= alpha;
               o[i][t][2 + e] *= alpha;
             }
+            d[t][e] = s[t][e] - m_new;
+            d[t][2 + e] = s[t][2 + e] - m_new;
           }
       }
       uint32_t pf[N][2];
 #pragma unroll
       for (int t = 0; t < N; ++t) {
-        // nothing seen yet: all weights 0
-        const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0] - C::HEADROOM;
-        const float m1 = m[t][1] == -INFINITY ? 0.f : m[t][1] - C::HEADROOM;
-        const float p0 = ex2_approx(s[t][0] - m0), p1 = ex2_approx(s[t][1] - m1);
-        const float p2 = ex2_approx(s[t][2] - m0), p3 = ex2_approx(s[t][3] - m1);
+        const float p0 = ex2_approx(d[t][0]), p1 = ex2_approx(d[t][1]);
+        const float p2 = ex2_approx(d[t][2]), p3 = ex2_approx(d[t][3]);
         l[t][0] += QUANT ? fmaf(p0, w0, p2 * w1) : p0 + p2;
         l[t][1] += QUANT ? fmaf(p1, w0, p3 * w1) : p1 + p3;
         // rounded for the product with V (bf16: half a step of 2^-8 relative for each probability)
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], x);
-        if (n == 0) ml_smem[copy0 + row0 + t * row_step + 2 * j + e] = make_float2(m[t][e], l[t][e]);
+        if (n == 0) ml_smem[copy0 + row0 + t * row_step + 2 * j + e] = make_float2(m_sub[t][e], l[t][e]);
       }
     __syncthreads();
 #pragma unroll
@@ -567,7 +573,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
         float mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < C::COPIES; ++w) mx = fmaxf(mx, ml_smem[w * C::ROWS + r].x);
-        const float f = m[t][e] == mx ? 1.f : ex2_approx(m[t][e] - mx);
+        const float f = ex2_approx(m_sub[t][e] - mx);
         float* dst = merge + (copy0 + r) * C::O_LD;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
