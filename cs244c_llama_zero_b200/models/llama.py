@@ -430,10 +430,12 @@ class LlamaForCausalLM(nn.Module):
             if prompt < 1 or prompt + max_new_tokens - 1 > self.cfg.max_seq_len:
                 raise ValueError(f"generate: a prompt of {prompt} and {max_new_tokens} new tokens do not fit "
                                  f"max_seq_len {self.cfg.max_seq_len} with a key/value cache")
-        out = torch.empty(batch, prompt + max_new_tokens, dtype=input_ids.dtype, device=input_ids.device)
+        if max_new_tokens <= 0:
+            return input_ids
+        out = torch.empty(batch, prompt + max_new_tokens, dtype=torch.int64, device=input_ids.device)
         out[:, :prompt] = input_ids
         cache = weights = None
-        if kv_cache is not None and max_new_tokens > 0:
+        if kv_cache is not None:
             from .kv_cache import PagedKVCache
 
             cache = PagedKVCache.for_batch(self.cfg, batch, prompt + max_new_tokens - 1, dtype=kv_cache,
@@ -458,7 +460,7 @@ class LlamaForCausalLM(nn.Module):
         def per_row(value, dtype):
             return torch.full((tokens.shape[0],), value, dtype=dtype, device=logits.device)
 
-        return B.adjust_logits(logits, tokens.long(), per_row(n, torch.int32), per_row(prompt, torch.int32),
+        return B.adjust_logits(logits, tokens, per_row(n, torch.int32), per_row(prompt, torch.int32),
                                per_row(repetition, torch.float32), per_row(frequency, torch.float32),
                                per_row(presence, torch.float32), bias, allowed)
 

@@ -55,4 +55,5 @@ def test_cached_generation_needs_the_b200_backend():
         model.generate(ids, 2, repetition_penalty=1.2)
     with pytest.raises(ValueError, match="b200 backend"):
         model.decode_weights()
-    assert model.generate(ids, 0).shape == (1, 4)
+    assert torch.equal(model.generate(ids, 0), ids) and torch.equal(model.generate(ids, -3), ids)
+    assert model.generate(ids.int(), 2, temperature=0.0).dtype == torch.int64
