@@ -243,23 +243,29 @@ std::vector<std::vector<int64_t>> paged_schedule(Tensor starts, Tensor lens, int
   std::vector<long long> base;
   for (int b = 0; b < s.batch; ++b) {
     base.push_back(total);
-    total += b200::head_units(b200::seq_info(s, b), shape) * kv_heads;
+    total += b200::head_places(b200::seq_info(s, b), shape) * kv_heads;
   }
   const long long blocks = std::min<long long>(grid, total);
-  for (long long c = 0; c < blocks; ++c) {
-    long long u = b200::range_begin(c, total, blocks);
-    const long long end = b200::range_begin(c + 1, total, blocks);
-    TORCH_CHECK(b200::block_of_unit(u, total, blocks) == c && b200::block_of_unit(end - 1, total, blocks) == c,
-                "paged_schedule: block_of_unit");
+  auto item_of = [&](long long v) {
     int b = s.batch - 1;
-    while (base[b] > u || b200::seq_info(s, b).qn == 0) --b;
-    b200::PagedItem it = b200::item_at(s, shape, b, base[b], u);
+    while (base[b] > v || b200::seq_info(s, b).qn == 0) --b;
+    return b200::item_at(s, shape, b, base[b], v);
+  };
+  auto cut = [&](long long c) {
+    if (c == blocks) return total;
+    const long long v = b200::raw_begin(c, total, blocks);
+    return b200::moved_cut(item_of(v), v);
+  };
+  for (long long c = 0; c < blocks; ++c) {
+    const long long begin = cut(c), end = cut(c + 1);
+    if (begin == end) continue;
+    b200::PagedItem it = item_of(begin);
+    int unit = b200::unit_of_cut(it, begin);
     while (true) {
-      const long long stop = std::min(end, it.start + it.n_units);
-      out.push_back({c, it.b, it.kvh, it.rt, u - it.start, stop - it.start, it.n_units});
-      u = stop;
-      if (u == end) break;
+      out.push_back({c, it.b, it.kvh, it.rt, unit, b200::unit_of_cut(it, end), it.n_units});
+      if (end <= b200::item_end(it)) break;
       b200::next_item(it, s, shape);
+      unit = 0;
     }
   }
   return out;

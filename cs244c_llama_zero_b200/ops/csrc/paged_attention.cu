@@ -198,10 +198,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
     ws.total[1] = range.blocks;
   }
   if ((int)blockIdx.x >= range.blocks) return;
-  const long long u_begin = range_begin(blockIdx.x, range.total, range.blocks);
-  int left = (int)(range_begin(blockIdx.x + 1, range.total, range.blocks) - u_begin);  // units to compute
-  PagedItem it = item_at(p.seqs, shape, range.b, range.base, u_begin);
-  if (threadIdx.x == 0) ws.records[blockIdx.x] = {it.start, it.n_units, it.b, it.kvh, it.rt};
+  PagedItem it = range.item;
+  if (threadIdx.x == 0) ws.records[blockIdx.x] = {range.begin, it.start, it.n_units, it.b, it.kvh, it.rt};
+  if (range.begin == range.end) return;
 
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   float* merge = reinterpret_cast<float*>(smem + kDecodeWarps * C::RING);
@@ -210,7 +209,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
 
   // ---- loads: a second walk over the same units, STAGES ahead
   PagedItem li = it;
-  int l_unit = (int)(u_begin - it.start), l_left = left;
+  int l_unit = unit_of_cut(li, range.begin), l_stop = unit_of_cut(li, range.end);  // of this item
+  bool loading = true;
   int l_visible = item_visible(li.seq, li.rt, shape.tile_tokens);
   uint32_t slot_in = ring;
   constexpr int PER_ROW = C::ROW_BYTES / 16;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
   };
   int page = page_of();
   auto load_unit = [&]() {
-    if (l_left > 0) {
+    if (loading) {
       const int t0 = l_unit * 64 + 16 * warp;
       int live = min(16, l_visible - t0);
       if (live > 0 && (page < 0 || page >= p.seqs.n_pages)) {
@@ -260,14 +260,16 @@ __global__ void __launch_bounds__(kDecodeThreads)
         }
       }
       slot_in = slot_in + C::STAGE == ring + C::RING ? ring : slot_in + C::STAGE;
-      if (--l_left > 0) {
-        if (++l_unit == li.n_units) {
+      if (++l_unit == l_stop) {
+        loading = range.end > item_end(li);
+        if (loading) {
           next_item(li, p.seqs, shape);
           l_unit = 0;
+          l_stop = unit_of_cut(li, range.end);
           l_visible = item_visible(li.seq, li.rt, shape.tile_tokens);
         }
-        page = page_of();
       }
+      if (loading) page = page_of();
     }
     cp_async_commit();
   };
@@ -332,9 +334,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
   uint32_t slot_out = BY_ROWS ? smem_u32(smem) : ring;
   int stage = 0;
   bool first = true;
-  int unit = (int)(u_begin - it.start);
+  int unit = unit_of_cut(it, range.begin);
   while (true) {  // one item, or the part of it in this block's range
-    const int seg = min(left, it.n_units - unit);
+    const int seg = unit_of_cut(it, range.end) - unit;
     const bool whole = seg == it.n_units;
     const int tok0 = it.rt * shape.tile_tokens;
     const int rows = min(shape.tile_tokens, it.seq.qn - tok0) * p.group;
@@ -550,8 +552,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
 
     // ---- join the warps
     const int q0 = it.seq.q0 + tok0, head0 = it.kvh * p.group;
-    left -= seg;
-    if (left > 0) {
+    const bool more = range.end > item_end(it);
+    if (more) {
       next_item(it, p.seqs, shape);
       load_q(it);
     }
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
         if (d == 0) ws.ml[(size_t)slot * C::ROWS + r] = make_float2(mx, sum);
       }
     }
-    if (left == 0) break;
+    if (!more) break;
     first = false;
     unit = 0;
     __syncthreads();  // the merge buffers are free
@@ -631,18 +633,11 @@ __global__ void __launch_bounds__(kJoinThreads)
   pdl_wait_and_release();
   constexpr int ROWS_AT_ONCE = kJoinThreads / 32 / WARPS_PER_ROW;
   constexpr int V = HD / 32;  // columns per lane
-  const int c = blockIdx.x + 1;
-  const long long total = ws.total[0];
-  const int blocks = (int)ws.total[1];
-  const PagedRecord rec = ws.records[c];  // there for every block, written by those with work
-  if (c >= blocks) return;
-  const long long u = range_begin(c, total, blocks);
-  if (rec.start == u) return;                                     // no item is cut here
-  if (range_begin(c - 1, total, blocks) > rec.start) return;      // cut before as well: another block's
-  const int last = block_of_unit(rec.start + rec.n_units - 1, total, blocks);
-  const int first_slot = 2 * (c - 1) + (range_begin(c - 1, total, blocks) == rec.start ? 0 : 1);
-  const int parts = last - (c - 1) + 1;
-  auto slot = [&](int i) { return i == 0 ? first_slot : 2 * (c - 1 + i); };
+  const PagedJoin join = find_join(ws, blockIdx.x + 1);
+  if (join.parts == 0) return;
+  const PagedRecord& rec = join.rec;
+  const int parts = join.parts;
+  auto slot = [&](int i) { return join.slot(i); };
   const SeqInfo seq = seq_info(p.seqs, rec.b);
   const int tok0 = rec.rt * shape.tile_tokens;
   const int rows = min(shape.tile_tokens, seq.qn - tok0) * p.group;

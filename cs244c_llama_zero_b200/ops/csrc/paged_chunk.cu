@@ -98,26 +98,24 @@ struct ChunkCfg {
 // in registers it would spill inside the hot loops of the softmax.
 struct ChunkWalk {
   PagedItem it;
-  int j0, j1;      // units of the item in this block's range
-  int left;        // units from j0 to the end of the range
+  long long end;   // of the block's range
+  int j0, j1;      // units of the item in it
   int n_tiles;     // 1: the item has rows in tile A only
   int visible;     // cached tokens that its last row sees
 };
-__device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh, int j0, int left) {
+__device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh, int j0) {
   w.j0 = j0;
-  w.left = left;
-  w.j1 = min(w.it.n_units, j0 + left);
+  w.j1 = unit_of_cut(w.it, w.end);
   w.n_tiles = w.it.seq.qn - w.it.rt * sh.tile_tokens > sh.tile_tokens / 2 ? 2 : 1;
   w.visible = item_visible(w.it.seq, w.it.rt, sh.tile_tokens);
 }
 // By one thread.  False at the end of the range.
 __device__ __forceinline__ bool next_part(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh) {
-  const int left = w.left - (w.j1 - w.j0);
-  if (left == 0) return false;
+  if (w.end <= item_end(w.it)) return false;
   PagedItem it = w.it;
   next_item(it, s, sh);
   w.it = it;
-  enter_item(w, sh, 0, left);
+  enter_item(w, sh, 0);
   return true;
 }
 // By a whole warp.
@@ -283,16 +281,17 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     ws.total[0] = range.total;
     ws.total[1] = range.blocks;
   }
-  const bool busy = (int)blockIdx.x < range.blocks;
+  const bool busy = range.begin != range.end;
   __shared__ ChunkWalk walks[C::THREADS / 32];
   ChunkWalk& w = walks[warp];
   if (busy && lane == 0) {
-    const long long u = range_begin(blockIdx.x, range.total, range.blocks);
-    const PagedItem it = item_at(p.seqs, shape, range.b, range.base, u);
-    w.it = it;
-    enter_item(w, shape, (int)(u - it.start), (int)(range_begin(blockIdx.x + 1, range.total, range.blocks) - u));
-    if (warp == 0) ws.records[blockIdx.x] = {it.start, it.n_units, it.b, it.kvh, it.rt};
+    w.it = range.item;
+    w.end = range.end;
+    enter_item(w, shape, unit_of_cut(range.item, range.begin));
   }
+  if ((int)blockIdx.x < range.blocks && threadIdx.x == 0)
+    ws.records[blockIdx.x] = {range.begin, range.item.start, range.item.n_units, range.item.b, range.item.kvh,
+                              range.item.rt};
   __syncwarp();
   const int tile_tokens = shape.tile_tokens / 2;  // of one tile
   const int page_log2 = p.seqs.page_log2;
@@ -847,16 +846,10 @@ template <int HD>
 __global__ void __launch_bounds__(kItemRows)
     paged_chunk_join_kernel(const __grid_constant__ PagedAttnParams p, PagedShape shape, PagedWorkspace ws) {
   pdl_wait_and_release();
-  const long long total = ws.total[0];
-  const int blocks = (int)ws.total[1];
-  const int c = blockIdx.x + 1;
-  if (c >= blocks) return;
-  const PagedRecord rec = ws.records[c];
-  const long long before = range_begin(c - 1, total, blocks);
-  if (rec.start == range_begin(c, total, blocks) || before > rec.start) return;
-  const int last = block_of_unit(rec.start + rec.n_units - 1, total, blocks);
-  const int parts = last - c + 2;
-  const int first_slot = 2 * (c - 1) + (before == rec.start ? 0 : 1);
+  const PagedJoin join = find_join(ws, blockIdx.x + 1);
+  if (join.parts == 0) return;
+  const PagedRecord& rec = join.rec;
+  const int parts = join.parts;
   const SeqInfo seq = seq_info(p.seqs, rec.b);
   const int tile_tokens = shape.tile_tokens / 2;
   const int row = threadIdx.x;
@@ -865,7 +858,7 @@ __global__ void __launch_bounds__(kItemRows)
   if (tok_in_tile >= tile_tokens || tok >= seq.qn) return;
   float mx = -INFINITY;
   for (int i = 0; i < parts; ++i) {
-    const int slot = i == 0 ? first_slot : 2 * (c - 1 + i);
+    const int slot = join.slot(i);
     mx = fmaxf(mx, ws.ml[(size_t)slot * kItemRows + row].x);
   }
   float4 acc[4];
@@ -873,7 +866,7 @@ __global__ void __launch_bounds__(kItemRows)
   for (int d = 0; d < 4; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
   for (int i = 0; i < parts; ++i) {
-    const int slot = i == 0 ? first_slot : 2 * (c - 1 + i);
+    const int slot = join.slot(i);
     const float2 q = ws.ml[(size_t)slot * kItemRows + row];
     const float f = q.x == mx ? 1.f : ex2_approx(q.x - mx);
     l += q.y * f;

@@ -142,7 +142,8 @@ def test_bad_logits(F):
                                                         (1, 6, 592)])
 @pytest.mark.parametrize("seed", range(4))
 def test_every_unit_is_done_once(F, tile_tokens, unit_log2, grid, seed):
-    """The blocks' ranges cover all units of all items once, in order, and differ by at most one unit."""
+    """The blocks' ranges cover all units of all items once, in order, and no block has more to do than its
+    share (units, and two places for each item that begins in it) and one item's start."""
     from cs244c_llama_zero_b200 import ops
 
     from tests.serving_reference import ragged
@@ -163,15 +164,21 @@ def test_every_unit_is_done_once(F, tile_tokens, unit_log2, grid, seed):
                 want.append((b, h, rt, max(1, -(-visible // (1 << unit_log2)))))
     got, sizes = [], {}
     for block, b, h, rt, u0, u1, units in parts:
-        sizes[block] = sizes.get(block, 0) + u1 - u0
+        sizes[block] = sizes.get(block, 0) + u1 - u0 + (2 if u0 == 0 else 0)
         assert 0 <= u0 < u1 <= units
         if u0 == 0:
             got.append([b, h, rt, 0])
         assert got[-1][:3] == [b, h, rt] and got[-1][3] == u0
         got[-1][3] = u1
     assert [tuple(g) for g in got] == want
-    assert sorted(sizes) == list(range(min(grid, sum(w[3] for w in want))))
-    assert max(sizes.values()) - min(sizes.values()) <= 1
+    total = sum(w[3] + 2 for w in want)
+    blocks = min(grid, total)
+    assert list(sizes) == sorted(sizes) and max(sizes) < blocks
+    assert max(sizes.values()) <= -(-total // blocks) + 2
+    # at most two parts per block, its first and its last one
+    for block in sizes:
+        cut = [i for i, p in enumerate(q for q in parts if q[0] == block) if p[5] - p[4] != p[6]]
+        assert set(cut) <= {0, sum(q[0] == block for q in parts) - 1}
 
 
 def test_bad_sequences_get_no_units(F):
