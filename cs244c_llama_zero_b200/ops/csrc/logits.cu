@@ -51,7 +51,7 @@ struct alignas(16) Vec {
 
 // Rows start anywhere: ranges are counted in 16-byte groups of the row's memory, `shift` elements of the first
 // group belonging to what lies before the row.  Steps that the row does not fill, and all steps when input and
-// output are aligned differently, go element by element.
+// output are aligned differently, go group by group, and element by element in groups that are not full.
 template <typename T, int NV, int RANGE, int MIN_BLOCKS>
 __global__ void __launch_bounds__(kThreads, MIN_BLOCKS) adjust_logits_kernel(LogitsParams p, unsigned blocks_per_row) {
   pdl_wait_and_release();
@@ -168,14 +168,24 @@ __global__ void __launch_bounds__(kThreads, MIN_BLOCKS) adjust_logits_kernel(Log
     const int at = base + step;
     if (at >= p.vocab) break;
     if (!whole(at)) {
-      for (int g = tid; g < SPAN; g += kThreads) {
-        const int t = at + g;
-        if (t < 0 || t >= p.vocab) continue;
-        float l = to_f32(src[t]);
-        if (penalise && ((seen[(step + g) >> 5] >> (g & 31)) & 1u)) l = __uint_as_float(counts[step + g]);
+      auto adjusted = [&](float l, int t) {
+        const int g = t - base;
+        if (penalise && ((seen[g >> 5] >> (g & 31)) & 1u)) l = __uint_as_float(counts[g]);
         if (bias != nullptr) l += bias[t];
         if (allowed != nullptr && !((allowed[t >> 5] >> (t & 31)) & 1u)) l = -INFINITY;
-        dst[t] = from_f32<T>(l);
+        return from_f32<T>(l);
+      };
+#pragma unroll 1
+      for (int t0 = at + tid * VE; t0 < min(at + SPAN, p.vocab); t0 += GROUPS) {
+        if (same && t0 >= 0 && t0 + VE <= p.vocab) {
+          Vec<T> y = *reinterpret_cast<const Vec<T>*>(src + t0);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) y.e[e] = adjusted(to_f32(y.e[e]), t0 + e);
+          *reinterpret_cast<Vec<T>*>(dst + t0) = y;
+        } else {
+#pragma unroll 1
+          for (int t = max(t0, 0); t < min(t0 + VE, p.vocab); ++t) dst[t] = adjusted(to_f32(src[t]), t);
+        }
       }
       continue;
     }
