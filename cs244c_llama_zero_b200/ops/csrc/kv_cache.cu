@@ -215,7 +215,6 @@ __global__ void __launch_bounds__(kThreads)
     }
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
-      if (at[i] < 0) continue;
       float f[8];
       if constexpr (FMT == KV_BF16) {
         unpack8(x[i], f);
@@ -244,10 +243,19 @@ __global__ void __launch_bounds__(kThreads)
         for (int e = 0; e < 8; ++e) f[e] *= sc[i];
       }
       if constexpr (F32) {
-        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at[i]);
-        dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-        dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-      } else {
+        // two lanes hold 64 bytes; they swap 16 so that each of their stores fills a 32-byte sector
+        const bool odd = lane & 1;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __shfl_xor_sync(0xffffffffu, odd ? f[e] : f[4 + e], 1);
+        if (at[i] >= 0) {
+          float* dst = reinterpret_cast<float*>(out) + at[i];
+          *reinterpret_cast<float4*>(odd ? dst - 4 : dst) =
+              odd ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<float4*>(odd ? dst + 4 : dst + 8) =
+              odd ? make_float4(f[4], f[5], f[6], f[7]) : make_float4(x[0], x[1], x[2], x[3]);
+        }
+      } else if (at[i] >= 0) {
         uint4 q;
         q.x = pack_bf16(f[0], f[1]);
         q.y = pack_bf16(f[2], f[3]);
