@@ -14,9 +14,10 @@
 // With 8-bit pages the products are taken in fp16, whose 11 bits lose nothing next to the result's 8: a row of q is
 // scaled by a power of two to a maximum in [1, 2), and code * scale of K and of V by one for each unit of 128
 // tokens (to a maximum in (2^14, 2^15]); a token's factor and its product with a code are rounded there (2^-12
-// relative each, for scales down to 2^-19 of the unit's largest).  K's power multiplies the unit's scores.  V's, 2^e, goes into the exponent: the weights are 2^(s_j + e - m), with the running maximum m taken
-// over s_j + e and 2^6 of headroom, and the normaliser sums them times 2^-e.  Rounding code * scale to bf16
-// instead cost two bits of the result.
+// relative each, for scales down to 2^-19 of the unit's largest).  K's power multiplies the unit's scores.  V's,
+// 2^e, goes into the exponent: the weights are 2^(s_j + e - m), with the running maximum m taken over s_j + e and
+// 2^6 of headroom, and the normaliser sums them times 2^-e.  Rounding code * scale to bf16 instead cost two bits of
+// the result.
 // That is for few tiles of a sequence.  With many (a long prompt), every tile would expand the same codes again:
 // then one kernel expands all visible units once, to fp16 [sequence, unit, kv head, 128, head_dim] with their
 // powers of two beside them, and Q's rows, and the attention kernel loads both by TMA (KV_EXPANDED).
