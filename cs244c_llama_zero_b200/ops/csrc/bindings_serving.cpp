@@ -83,6 +83,8 @@ b200::KvPool check_pool(const Tensor& k, const Tensor& v, const std::optional<Te
     for (const Tensor* s : {&*ks, &*vs})
       TORCH_CHECK(s->scalar_type() == at::kFloat && s->is_contiguous() && s->sizes() == k.sizes().slice(0, 3),
                   "scales must be contiguous float32 [n_pages, kv_heads, page_size]");
+    check_aligned(*ks, "k_scale");
+    check_aligned(*vs, "v_scale");
     p.k_scale = ks->data_ptr<float>();
     p.v_scale = vs->data_ptr<float>();
   }

@@ -269,7 +269,8 @@ class KVPages(NamedTuple):
 
     ``k`` and ``v`` are pools of pages ``[n_pages, kv_heads, page_size, head_dim]`` (contiguous, page_size
     16, 32, 64 or 128) in bfloat16, or in 8 bits (float8_e4m3fn or int8) with one float32 scale per token
-    and head in ``k_scale`` / ``v_scale`` ``[n_pages, kv_heads, page_size]``: a row ``x`` is stored as
+    and head in ``k_scale`` / ``v_scale`` ``[n_pages, kv_heads, page_size]`` (contiguous; pages and scales
+    start on 16-byte boundaries): a row ``x`` is stored as
     ``scale = max|x| / M`` and ``code = round(x * M / max|x|)`` with M = 448 (e4m3) or 127 (int8).  A row
     with an infinity or a NaN gets the scale NaN and reads back as NaN.  Scales are never negative.
 
