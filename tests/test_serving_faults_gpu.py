@@ -1,0 +1,72 @@
+"""Corners of the serving operators on the GPU, against their 64-bit definitions: rows and units of zeros, values of
+extreme size, infinities and NaN in places that a row does not see, scratch memory that is not to be had."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.serving_bounds import bound, norm_bound
+from tests.serving_reference import FORMATS, Batch
+
+pytestmark = pytest.mark.gpu
+
+QUANTISED = ["e4m3", "int8"]
+# (heads, kv heads, head size), new tokens: few rows, few rows split over the warps, a chunk whose codes are expanded
+# in its tiles, one long enough that they are expanded once
+FORMS = [((8, 2, 64), 3), ((8, 2, 64), 14), ((8, 2, 64), 60), ((8, 2, 64), 150),
+         ((16, 8, 128), 4), ((16, 8, 128), 60), ((16, 8, 128), 150)]
+
+
+@pytest.fixture(scope="module")
+def F():
+    from cs244c_llama_zero_b200 import ops
+    from cs244c_llama_zero_b200.ops import functional
+
+    ops.load_extension().reset_device_errors()
+    yield functional
+    ops.check_device_errors()
+
+
+def _attend(F, b, **kw):
+    return F.paged_attention(b.q.cuda(), b.pages("cuda"), b.table.cuda(), b.lens.cuda(), b.starts.cuda(), b.max_q, **kw)
+
+
+def _attend_many(F, b, copies=24, **kw):
+    """The batch ``copies`` times over the same pages, so that a block's range holds several units of an item."""
+    starts = torch.cat([b.starts[:1]] + [b.starts[1:] + i * b.total for i in range(copies)])
+    out = F.paged_attention(b.q.repeat(copies, 1, 1).cuda(), b.pages("cuda"), b.table.repeat(copies, 1).cuda(),
+                            b.lens.repeat(copies).cuda(), starts.cuda(), b.max_q, **kw)
+    return out.view(copies, *b.q.shape)
+
+
+def _check(got, b, want=None, rows=slice(None), **kw):
+    want, mag, size = b.attention(**kw) if want is None else want
+    got = got[:b.total].double().cpu()
+    far = ~((got - want).abs() <= bound(want, mag, size, b.fmt))
+    far = far[rows]
+    assert not far.any(), (f"{int(far.sum())} of {far.numel()} outside, first at {far.nonzero()[0].tolist()}: "
+                           f"{got[rows][far][0]} for {want[rows][far][0]}")
+
+
+# ------------------------------------------------------------------------------------------ precision
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
+def test_rounding_of_ordinary_activations(F, fmt, heads, q_len):
+    """Element by element inside the bound of the form's own roundings, and as a whole near what they add up to."""
+    b = Batch([q_len, 1, q_len], [q_len + 700, 333, q_len], *heads, fmt, 64, seed=45)
+    want, mag, size = b.attention()
+    got = _attend(F, b)
+    _check(got, b, (want, mag, size))
+    error = (got.double().cpu() - want).norm() / want.norm()
+    assert error <= norm_bound(fmt), float(error)
+
+
+@pytest.mark.parametrize("fmt", QUANTISED)
+@pytest.mark.parametrize("heads,q_len", FORMS)
+def test_scales_of_different_size_in_a_unit(F, fmt, heads, q_len):
+    """Every seventh token's K 2^12 times smaller and V 2^12 times larger than the others'."""
+    b = Batch([q_len, 3], [q_len + 400, 90], *heads, fmt, 16, seed=46)
+    b.scales[0][:, :, ::7] *= 2.0 ** -12
+    b.scales[1][:, :, ::7] *= 2.0 ** 12
+    _check(_attend(F, b), b)
