@@ -66,6 +66,22 @@ __host__ __device__ inline int seq_of_row(const PagedSeqs& s, int t) {
   return lo;
 }
 
+#if defined(__CUDACC__)
+
+// Biased exponent of the power of two that a row of q is divided by before it becomes fp16, from the largest |x| of
+// the row (bf16 bits): the row's maximum lands in [1, 2).  A row of zeros is left alone: with the smallest
+// power, its product with the scale and K's power could reach 0, and a masked score, -inf, times 0 is NaN.
+__device__ __forceinline__ int q_row_exponent(uint32_t top) {
+  return top == 0u ? 127 : min(max((int)(top >> 7), 2), 252);
+}
+// What the scores of such a row are multiplied by, kept a positive number (-inf stays -inf, 0 stays 0): where the
+// product leaves the range of fp32 at the lower end, the scores are 0 to fp32 all the same.
+__device__ __forceinline__ float score_factor(float scale, float q_power, float k_power) {
+  return fminf(fmaxf(scale * q_power * k_power, 1.17549435e-38f), 3.40282347e38f);
+}
+
+#endif
+
 struct KvPool {
   void* k;
   void* v;

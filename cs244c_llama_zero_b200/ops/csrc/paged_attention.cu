@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
         uint32_t m = max(top & 0xFFFFu, top >> 16);
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int e = min(max((int)(m >> 7), 2), 252);  // biased exponent of the row's maximum
+        const int e = q_row_exponent(m);
         const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)

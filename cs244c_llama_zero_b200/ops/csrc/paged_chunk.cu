@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
             top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
                                          __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
           }
-          const int e = min(max((int)(max(top & 0xFFFFu, top >> 16) >> 7), 2), 252);  // biased exponent of the maximum
+          const int e = q_row_exponent(max(top & 0xFFFFu, top >> 16));
           const float down = __uint_as_float((uint32_t)(254 - e) << 23);
           reinterpret_cast<float*>(smem + C::UNIT_OFF)[(qs * 2 + t) * 128 + tid] = __uint_as_float((uint32_t)e << 23);
           uint8_t* row = smem + C::Q_OFF + qs * 2 * C::TILE_BYTES + t * C::TILE_BYTES + tid * 128;
@@ -669,14 +669,14 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           // scores to log2 units; 8-bit: plus V's exponent
           float to_log2 = scale2, v_exp = 0.f;
           if constexpr (C::EXPANDED) {
-            to_log2 = scale2 * q_power * power.x;
+            to_log2 = score_factor(scale2, q_power, power.x);
             v_exp = power.y;
             if (j + 1 < j1) power = powers[(long long)(j + 1) * shape.kv_heads];  // for the next unit
           }
           if constexpr (C::QUANT) {
             const float* units = reinterpret_cast<const float*>(smem + C::UNIT_OFF);
             const float2 u = reinterpret_cast<const float2*>(units + C::Q_BUFS * 256)[(g + j - j0) % C::STAGES];
-            to_log2 = scale2 * units[((part_no % C::Q_BUFS) * 2 + t) * 128 + r] * u.x;
+            to_log2 = score_factor(scale2, units[((part_no % C::Q_BUFS) * 2 + t) * 128 + r], u.x);
             v_exp = u.y;
           }
           uint32_t s[C::QUANT ? 2 : 4][32];  // 8-bit: two buffers of 32 scores, else the row's 128
@@ -914,7 +914,7 @@ __global__ void __launch_bounds__(128) paged_expand_kernel(PagedAttnParams p, Ex
     const uint32_t group = LANES == 32 ? 0xFFFFFFFFu : ((1u << LANES) - 1u) << (lane / LANES * LANES);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(group, m, o));
-    const int e = min(max((int)(m >> 7), 2), 252);  // biased exponent of the row's maximum
+    const int e = q_row_exponent(m);
     const float down = __uint_as_float((uint32_t)(254 - e) << 23);
     uint4 y;
     y.x = pack_f16(bf16lo(x.x) * down, bf16hi(x.x) * down);

@@ -49,6 +49,24 @@ def _check(got, b, want=None, rows=slice(None), **kw):
                            f"{got[rows][far][0]} for {want[rows][far][0]}")
 
 
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("heads,q_len", FORMS)
+@pytest.mark.parametrize("k_size,scale", [(2.0 ** -14, None), (1.0, 1e-4), (2.0 ** -60, 1e-20)])
+def test_zero_query_rows(F, fmt, heads, q_len, k_size, scale):
+    """A row of zeros has equal scores: the mean of the visible V, however small K and the scale are."""
+    b = Batch([q_len, 2], [q_len + 70, 40], *heads, fmt, 16, seed=40)
+    b.q[::3] = 0
+    b.q[1, :1] = 0
+    if fmt == "bf16":
+        b.pools[0] = (b.pools[0].float() * k_size).to(torch.bfloat16)
+    else:
+        b.scales[0] *= k_size
+    want = b.attention(scale=scale)
+    _check(_attend(F, b, scale=scale), b, want)
+    for got in _attend_many(F, b, scale=scale):
+        _check(got, b, want)
+
+
 # ------------------------------------------------------------------------------------------ precision
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
