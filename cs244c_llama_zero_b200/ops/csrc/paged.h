@@ -80,6 +80,12 @@ __device__ __forceinline__ float score_factor(float scale, float q_power, float 
   return fminf(fmaxf(scale * q_power * k_power, 1.17549435e-38f), 3.40282347e38f);
 }
 
+// V that is all zero adds nothing to a row but its weights' sum.  Where V's size goes into the exponent of the
+// weights it gets the lowest one: any size of its own could raise the maximum so far above the others' exponents
+// that their fp16 weights sink into subnormals.  Not lower than this, so that weights of up to 2^14 times
+// 2^80, summed over 2^31 tokens, stay below 2^126.
+constexpr int kLowestExponent = -80;
+
 #endif
 
 struct KvPool {

@@ -153,12 +153,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// 2^e, and the exponent e that brings max_code * scale into (2^14, 2^15] (0 for a scale of 0).
+// 2^e, and the exponent e that brings max_code * scale into (2^14, 2^15] (the lowest one for a scale of 0).
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int unit_exponent(uint32_t scale_bits, float max_code) {
-  if (scale_bits == 0u) return 0;
+  if (scale_bits == 0u) return kLowestExponent;
   const int e = (int)(__float_as_uint(__uint_as_float(scale_bits) * max_code) >> 23) - 127;  // floor(log2)
-  return min(max(e - 14, -100), 100);
+  return min(max(e - 14, kLowestExponent), 100);
 }
 
 template <int FMT>

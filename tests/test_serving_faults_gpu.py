@@ -67,6 +67,29 @@ def test_zero_query_rows(F, fmt, heads, q_len, k_size, scale):
         _check(got, b, want)
 
 
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("heads,q_len", FORMS)
+@pytest.mark.parametrize("v_size", [1.0, 2.0 ** -8, 2.0 ** -18, 2.0 ** -60])
+def test_units_whose_values_are_zero(F, fmt, heads, q_len, v_size):
+    """The first 192 tokens have V = 0 (and, in sequence 1, all): they count in the sum of the weights only, whatever
+    size the V behind them has, and also where their scores are the larger ones."""
+    b = Batch([q_len, q_len], [q_len + 330, 300], *heads, fmt, 32, seed=41)
+    for s, n in ((0, 192), (1, 300)):
+        for t in range(n):
+            at = b.table[s, t // 32], t % 32
+            b.pools[1][at[0], :, at[1]] = 0
+            if fmt != "bf16":
+                b.scales[1][at[0], :, at[1]] = 0
+    if fmt == "bf16":
+        b.pools[1] = (b.pools[1].float() * v_size).to(torch.bfloat16)
+    else:
+        b.scales[1] *= v_size
+    want = b.attention()
+    _check(_attend(F, b), b, want)
+    for got in _attend_many(F, b):
+        _check(got, b, want)
+
+
 # ------------------------------------------------------------------------------------------ precision
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
