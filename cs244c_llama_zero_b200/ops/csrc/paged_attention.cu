@@ -48,6 +48,8 @@ constexpr float kRaise = 8.0f;  // log2 units
 // The running maximum of a row that has seen nothing: finite, so that differences with it are numbers, and below
 // every score.
 constexpr float kNothing = -3.0e38f;
+constexpr float kZeroScale = 8.2718061e-25f;  // 2^kLowestExponent
+static_assert(kLowestExponent == -80, "kZeroScale");
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr int kUnitLog2 = 6;  // 16 tokens per warp
@@ -412,9 +414,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
       if constexpr (QUANT) {
         const uint32_t sa = tile + 2 * C::TILE + n * 4;
         const float k0 = lds32f(sa), k1 = lds32f(sa + 32), v0 = lds32f(sa + 64), v1 = lds32f(sa + 96);
-        // a scale of 0 (all codes 0) counts as 2^-100; a NaN stays one
-        const float x0 = lg2_approx(fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
-        const float x1 = lg2_approx(fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
+        // a scale of 0 (all codes 0) counts as 2^kLowestExponent, one below 2^-100 as that; a NaN stays one
+        const float x0 = lg2_approx(v0 == 0.f ? kZeroScale : fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
+        const float x1 = lg2_approx(v1 == 0.f ? kZeroScale : fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
         w0 = ex2_approx(-x0);
         w1 = ex2_approx(-x1);
 #pragma unroll

@@ -90,6 +90,32 @@ def test_units_whose_values_are_zero(F, fmt, heads, q_len, v_size):
         _check(got, b, want)
 
 
+@pytest.mark.parametrize("fmt", QUANTISED)
+def test_many_values_of_zero(F, fmt):
+    """Tens of thousands of zero V in one block's range, ahead of others, with scores that rise by less than makes
+    the running maximum follow: the sum of their weights stays in range.  (The sequences share their pages.)"""
+    page, n, batch = 128, 32768, 512
+    pages = n // page
+    code = torch.full((pages, 1, page, 64), 127, dtype=torch.int8)
+    k = code.clone() if fmt == "int8" else code.float().to(torch.float8_e4m3fn)
+    unit = float(k.float().max())
+    k_scale = torch.full((pages, 1, page), 1.0 / unit)  # k = 1
+    k_scale[0, 0, :64] = 1e-6  # the first scores are next to 0, the others 7.9 / log2(e)
+    v = k.clone()
+    v_scale = torch.zeros(pages, 1, page)
+    v_scale[-1, 0, -32:] = 1.0 / unit  # the last 32 values are 1
+    cache = F.KVPages(*[t.cuda() for t in (k, v, k_scale, v_scale)])
+    q = torch.full((batch, 1, 64), 1.0, dtype=torch.bfloat16).cuda()
+    table = torch.arange(pages, dtype=torch.int32).expand(batch, pages).contiguous().cuda()
+    lens = torch.full((batch,), n, dtype=torch.int32).cuda()
+    score = 7.9 * 0.6931471805599453
+    out = F.paged_attention(q, cache, table, lens, scale=score / 64).double().cpu()
+    low = torch.exp(torch.tensor(-score * (1 - 1e-6 * unit), dtype=torch.float64))
+    want = 32 / (n - 64 + 64 * low)
+    # the result's rounding, the weights' (fp16), and scores of 8 in fp32
+    assert ((out - want).abs() <= want * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -16)).all(), (out.min(), out.max(), want)
+
+
 # ------------------------------------------------------------------------------------------ precision
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
