@@ -158,7 +158,7 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 __device__ __forceinline__ int unit_exponent(uint32_t scale_bits, float max_code) {
   if (scale_bits == 0u) return kLowestExponent;
   const int e = (int)(__float_as_uint(__uint_as_float(scale_bits) * max_code) >> 23) - 127;  // floor(log2)
-  return min(max(e - 14, kLowestExponent), 100);
+  return max(e - 14, kLowestExponent);  // (113 for the largest bf16 values)
 }
 
 template <int FMT>

@@ -116,6 +116,16 @@ def test_many_values_of_zero(F, fmt):
     assert ((out - want).abs() <= want * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -16)).all(), (out.min(), out.max(), want)
 
 
+@pytest.mark.parametrize("fmt", QUANTISED)
+@pytest.mark.parametrize("heads,q_len", FORMS)
+@pytest.mark.parametrize("exponent", [110, 121])
+def test_values_of_huge_size(F, fmt, heads, q_len, exponent):
+    """V up to 2^(exponent + 4): no factor on the way leaves its type's range."""
+    b = Batch([q_len], [q_len + 200], *heads, fmt, 16, seed=42)
+    b.scales[1] *= 2.0 ** exponent
+    _check(_attend(F, b), b)
+
+
 # ------------------------------------------------------------------------------------------ precision
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
