@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <optional>
@@ -191,7 +192,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   }
   TORCH_CHECK(max_q >= 1 && max_q <= INT_MAX, "max_q_len must be at least 1");
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)pool.head_dim);
-  TORCH_CHECK(scale > 0.0 && scale <= 1e30, "scale must be positive and finite");
+  TORCH_CHECK(scale >= FLT_MIN && scale <= 1e30, "scale must be between 2^-126 and 1e30");
   const b200::PagedSeqs seqs = check_seqs(k_pages, table, lens, starts, q.size(0), max_q);
   check_device(q, q, "q");
   if (out_.has_value()) check_device(*out_, q, "out");

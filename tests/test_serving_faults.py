@@ -42,3 +42,13 @@ def test_scales_off_a_16_byte_boundary_are_refused(F, which, by):
             call(bad)
         with pytest.raises(RuntimeError, match="must be a CUDA tensor"):  # 16 bytes further on they pass
             call(pages._replace(**{which: _moved(getattr(pages, which), 4)}))
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-39, 0.0, -1.0, 1e31, float("inf"), float("nan")])
+def test_scales_that_fp32_cannot_hold_are_refused(F, scale):
+    """The kernels multiply in fp32: what is 0 or not normal there is refused, not passed on as 0."""
+    b = Batch([2, 1], [5, 17], 4, 2, 64, "bf16", 16)
+    with pytest.raises(RuntimeError, match="scale must be"):
+        F.paged_attention(b.q, b.pages(), b.table, b.lens, b.starts, b.max_q, scale=scale)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        F.paged_attention(b.q, b.pages(), b.table, b.lens, b.starts, b.max_q, scale=2.0 ** -126)
