@@ -380,7 +380,13 @@ class LlamaForCausalLM(nn.Module):
         longest = max(cache.length(s) + n for s, n in zip(seqs, rows))
         if longest > self.cfg.max_seq_len:
             raise ValueError(f"decode_step: {longest} tokens exceed max_seq_len {self.cfg.max_seq_len}")
+        mine, theirs = ((c.n_layers, c.n_kv_heads, c.head_dim) for c in (self.cfg, cache.cfg))
+        if mine != theirs:
+            raise ValueError(f"decode_step: the cache is one of {theirs} layers, kv heads and head_dim, "
+                             f"the model has {mine}")
         weights = self.decode_weights() if weights is None else weights
+        if len(weights) != len(self.layers):
+            raise ValueError(f"decode_step: weights of {len(weights)} blocks for {len(self.layers)} layers")
         batch = cache.extend(seqs, rows)
         cos, sin = (t[:, batch.positions].contiguous() for t in B.rope_tables_t(
             self.cfg.max_seq_len, self.cfg.head_dim, self.cfg.rope_theta, input_ids.device))

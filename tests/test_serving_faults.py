@@ -52,3 +52,52 @@ def test_scales_that_fp32_cannot_hold_are_refused(F, scale):
         F.paged_attention(b.q, b.pages(), b.table, b.lens, b.starts, b.max_q, scale=scale)
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         F.paged_attention(b.q, b.pages(), b.table, b.lens, b.starts, b.max_q, scale=2.0 ** -126)
+
+
+# ------------------------------------------------------------------------------------------ decoding over a cache
+def _model(**kw):
+    """A model whose decode_step runs on the CPU up to the first kernel."""
+    from cs244c_llama_zero_b200.models import LlamaForCausalLM, ModelConfig
+
+    args = dict(name="t", vocab_size=97, max_seq_len=64, dim=256, n_layers=3, n_heads=4, n_kv_heads=2, ffn_dim=256)
+    model = LlamaForCausalLM(ModelConfig(**{**args, **kw})).eval()
+    model.backend = "b200"
+    return model
+
+
+def _cache(model, **kw):
+    from cs244c_llama_zero_b200.models import PagedKVCache
+
+    args = {**model.cfg.__dict__, **kw}
+    return PagedKVCache.for_batch(type(model.cfg)(**args), 2, 40, page_size=16, device="cpu")
+
+
+@pytest.mark.parametrize("change", [dict(n_layers=2), dict(n_layers=4), dict(n_kv_heads=1), dict(dim=512)])
+def test_a_cache_of_another_model_is_refused(F, monkeypatch, change):
+    """Fewer layers in the cache than in the model would leave the model's last ones out."""
+    monkeypatch.setattr(F, "decode_block", lambda x, *a: x)
+    model = _model()
+    cache = _cache(model, **change)
+    ids = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="decode_step: the cache"):
+        model.decode_step(ids, cache, [0, 1], [2, 1], [None] * 3)
+    assert cache.length(0) == 0 and cache.free_pages == 6
+
+
+@pytest.mark.parametrize("count", [0, 2, 4])
+def test_weights_of_other_layers_are_refused(F, monkeypatch, count):
+    monkeypatch.setattr(F, "decode_block", lambda x, *a: x)
+    model = _model()
+    with pytest.raises(ValueError, match="decode_step: weights"):
+        model.decode_step(torch.zeros(3, dtype=torch.int64), _cache(model), [0, 1], [2, 1], [None] * count)
+
+
+def test_every_layer_runs_once(F, monkeypatch):
+    seen = []
+    monkeypatch.setattr(F, "decode_block", lambda x, w, cfg, pages, *a: seen.append((w, pages)) or x)
+    model = _model()
+    cache = _cache(model)
+    logits = model.decode_step(torch.zeros(3, dtype=torch.int64), cache, [0, 1], [2, 1], list("abc"))
+    assert logits.shape == (2, 97)
+    assert [w for w, _ in seen] == list("abc") and all(p is q for (_, p), q in zip(seen, cache.layers))
+    assert cache.length(0) == 2 and cache.length(1) == 1
