@@ -98,17 +98,32 @@ class PagedKVCache:
         need = [max(0, -(-(self._lens[s] + n) // self.page_size) - len(self._pages[s])) for s, n in zip(seqs, rows)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"the cache is out of pages: {sum(need)} needed, {len(self._free)} free")
+        # described first, taken when nothing can fail any more
+        left = len(self._free)
+        pages, lens = [], []
         for s, n, count in zip(seqs, rows, need):
-            self._pages[s].extend(self._free.pop() for _ in range(count))
-            self._lens[s] += n
-        width = max([len(self._pages[s]) for s in seqs] + [1])
-        table = torch.zeros(len(seqs), width, dtype=torch.int32)
-        for i, s in enumerate(seqs):
-            table[i, :len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
-        lens = torch.tensor([self._lens[s] for s in seqs], dtype=torch.int32)
+            pages.append(self._pages[s] + self._free[left - count:left][::-1])
+            lens.append(self._lens[s] + n)
+            left -= count
+        table = torch.zeros(len(seqs), max([len(p) for p in pages] + [1]), dtype=torch.int32)
+        for i, p in enumerate(pages):
+            table[i, :len(p)] = torch.tensor(p, dtype=torch.int32)
         starts = torch.zeros(len(seqs) + 1, dtype=torch.int32)
         starts[1:] = torch.cumsum(torch.tensor(list(rows), dtype=torch.int32), 0)
-        positions = torch.cat([torch.arange(self._lens[s] - n, self._lens[s]) for s, n in zip(seqs, rows)])
+        positions = torch.cat([torch.arange(end - n, end) for end, n in zip(lens, rows)])
         single = all(n == 1 for n in rows)
-        return CacheBatch(table.to(self.device), lens.to(self.device), None if single else starts.to(self.device),
-                          max(max(rows), 1), positions.to(self.device))
+        batch = CacheBatch(table.to(self.device), torch.tensor(lens, dtype=torch.int32).to(self.device),
+                           None if single else starts.to(self.device), max(max(rows), 1), positions.to(self.device))
+        for s, p, n in zip(seqs, pages, lens):
+            self._pages[s], self._lens[s] = p, n
+        del self._free[left:]
+        return batch
+
+    def retract(self, seqs: Sequence[int], rows: Sequence[int]) -> None:
+        """Takes the last ``rows[i]`` tokens off sequence ``seqs[i]``: undoes an :meth:`extend` whose step failed."""
+        if len(seqs) != len(rows) or any(not 0 <= n <= self._lens[s] for s, n in zip(seqs, rows)):
+            raise ValueError("retract: one row count for each sequence, of tokens that it has")
+        for s, n in reversed(list(zip(seqs, rows))):
+            self._lens[s] -= n
+            while len(self._pages[s]) > -(-self._lens[s] // self.page_size):
+                self._free.append(self._pages[s].pop())

@@ -370,7 +370,8 @@ class LlamaForCausalLM(nn.Module):
 
         ``input_ids`` [sum(rows)] holds ``rows[i]`` new tokens of cached sequence ``seqs[i]``, one sequence
         after the other: prompts, chunks of prompts or single tokens in any mixture.  Their keys and values
-        are added to ``cache``.  ``weights``: :meth:`decode_weights`, to lay them out once for many steps.
+        are added to ``cache``; a step that is refused leaves its lengths and pages as they were.  ``weights``:
+        :meth:`decode_weights`, to lay them out once for many steps.
         """
         from ..ops import functional as B
 
@@ -388,14 +389,18 @@ class LlamaForCausalLM(nn.Module):
         if len(weights) != len(self.layers):
             raise ValueError(f"decode_step: weights of {len(weights)} blocks for {len(self.layers)} layers")
         batch = cache.extend(seqs, rows)
-        cos, sin = (t[:, batch.positions].contiguous() for t in B.rope_tables_t(
-            self.cfg.max_seq_len, self.cfg.head_dim, self.cfg.rope_theta, input_ids.device))
-        x = self.tok_embeddings(input_ids)
-        for w, pages in zip(weights, cache.layers):
-            x = B.decode_block(x, w, self.cfg, pages, batch, cos, sin)
-        if batch.q_starts is not None:
-            x = x[(batch.q_starts[1:] - 1).long()]
-        return self.lm_head(self.norm(x))
+        try:
+            cos, sin = (t[:, batch.positions].contiguous() for t in B.rope_tables_t(
+                self.cfg.max_seq_len, self.cfg.head_dim, self.cfg.rope_theta, input_ids.device))
+            x = self.tok_embeddings(input_ids)
+            for w, pages in zip(weights, cache.layers):
+                x = B.decode_block(x, w, self.cfg, pages, batch, cos, sin)
+            if batch.q_starts is not None:
+                x = x[(batch.q_starts[1:] - 1).long()]
+            return self.lm_head(self.norm(x))
+        except BaseException:
+            cache.retract(seqs, rows)
+            raise
 
     def decode_weights(self) -> List[Any]:
         """Every block's weights as :meth:`decode_step` reads them (q|k|v and gate|up fused)."""

@@ -101,3 +101,35 @@ def test_every_layer_runs_once(F, monkeypatch):
     assert logits.shape == (2, 97)
     assert [w for w, _ in seen] == list("abc") and all(p is q for (_, p), q in zip(seen, cache.layers))
     assert cache.length(0) == 2 and cache.length(1) == 1
+
+
+def _state(cache):
+    return cache.free_pages, list(cache._free), [list(p) for p in cache._pages], [cache.length(s) for s in range(2)]
+
+
+@pytest.mark.parametrize("where", ["first", "last", "positions"])
+def test_a_step_that_fails_leaves_the_cache_as_it_was(F, monkeypatch, where):
+    """Whatever refuses a step, the tokens that it did not compute are not counted as cached."""
+    model = _model()
+    cache = _cache(model)
+    monkeypatch.setattr(F, "decode_block", lambda x, *a: x)
+    model.decode_step(torch.zeros(18, dtype=torch.int64), cache, [0, 1], [15, 3], [None] * 3)
+    before = _state(cache)
+    calls = []
+
+    def block(x, *a):
+        calls.append(1)
+        if where == "first" or len(calls) == 3:
+            raise RuntimeError("refused")
+        return x
+
+    monkeypatch.setattr(F, "decode_block", block)
+    if where == "positions":
+        def tables(*a):
+            raise RuntimeError("refused")
+        monkeypatch.setattr(F, "rope_tables_t", tables)
+    with pytest.raises(RuntimeError, match="refused"):
+        model.decode_step(torch.zeros(19, dtype=torch.int64), cache, [1, 0], [14, 5], [None] * 3)
+    assert _state(cache) == before
+    step = cache.extend([0, 1], [1, 1])  # and it goes on from there
+    assert step.kv_lens.tolist() == [16, 4] and step.positions.tolist() == [15, 3]
