@@ -79,11 +79,18 @@ class PagedKVCache:
         self._lens.append(0)
         return len(self._lens) - 1
 
+    def _check(self, seqs: Sequence[int]) -> None:
+        for s in seqs:
+            if not 0 <= s < len(self._lens):
+                raise IndexError(f"the cache has no sequence {s}, only 0 to {len(self._lens) - 1}")
+
     def length(self, seq: int) -> int:
+        self._check([seq])
         return self._lens[seq]
 
     def release(self, seq: int) -> None:
         """Returns the sequence's pages; it is empty afterwards."""
+        self._check([seq])
         self._free.extend(reversed(self._pages[seq]))
         self._pages[seq] = []
         self._lens[seq] = 0
@@ -93,6 +100,7 @@ class PagedKVCache:
         Nothing is changed if the pool has too few pages."""
         if len(seqs) != len(rows) or len(set(seqs)) != len(seqs):
             raise ValueError("extend: one row count for each of a set of different sequences")
+        self._check(seqs)
         if any(n < 0 for n in rows):
             raise ValueError("extend: row counts must not be negative")
         need = [max(0, -(-(self._lens[s] + n) // self.page_size) - len(self._pages[s])) for s, n in zip(seqs, rows)]
@@ -121,6 +129,7 @@ class PagedKVCache:
 
     def retract(self, seqs: Sequence[int], rows: Sequence[int]) -> None:
         """Takes the last ``rows[i]`` tokens off sequence ``seqs[i]``: undoes an :meth:`extend` whose step failed."""
+        self._check(seqs)
         if len(seqs) != len(rows) or any(not 0 <= n <= self._lens[s] for s, n in zip(seqs, rows)):
             raise ValueError("retract: one row count for each sequence, of tokens that it has")
         for s, n in reversed(list(zip(seqs, rows))):

@@ -133,3 +133,18 @@ def test_a_step_that_fails_leaves_the_cache_as_it_was(F, monkeypatch, where):
     assert _state(cache) == before
     step = cache.extend([0, 1], [1, 1])  # and it goes on from there
     assert step.kv_lens.tolist() == [16, 4] and step.positions.tolist() == [15, 3]
+
+
+@pytest.mark.parametrize("seq", [-1, -2, 2, 100])
+def test_sequences_that_do_not_exist_are_refused(F, seq):
+    """A negative number is not the sequence counted from the end: -1 and 1 would be one sequence twice."""
+    model = _model()
+    cache = _cache(model)
+    cache.extend([0, 1], [17, 3])
+    before = _state(cache)
+    for call in (lambda: cache.length(seq), lambda: cache.release(seq), lambda: cache.extend([seq], [1]),
+                 lambda: cache.extend([1, seq], [1, 1]), lambda: cache.retract([seq], [1]),
+                 lambda: model.decode_step(torch.zeros(2, dtype=torch.int64), cache, [1, seq], [1, 1], [None] * 3)):
+        with pytest.raises(IndexError, match="no sequence"):
+            call()
+    assert _state(cache) == before
