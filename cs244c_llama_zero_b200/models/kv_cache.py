@@ -130,8 +130,10 @@ class PagedKVCache:
     def retract(self, seqs: Sequence[int], rows: Sequence[int]) -> None:
         """Takes the last ``rows[i]`` tokens off sequence ``seqs[i]``: undoes an :meth:`extend` whose step failed."""
         self._check(seqs)
-        if len(seqs) != len(rows) or any(not 0 <= n <= self._lens[s] for s, n in zip(seqs, rows)):
-            raise ValueError("retract: one row count for each sequence, of tokens that it has")
+        if len(seqs) != len(rows) or len(set(seqs)) != len(seqs):
+            raise ValueError("retract: one row count for each of a set of different sequences")
+        if any(not 0 <= n <= self._lens[s] for s, n in zip(seqs, rows)):
+            raise ValueError("retract: a sequence has fewer tokens")
         for s, n in reversed(list(zip(seqs, rows))):
             self._lens[s] -= n
             while len(self._pages[s]) > -(-self._lens[s] // self.page_size):

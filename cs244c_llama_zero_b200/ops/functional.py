@@ -289,8 +289,8 @@ class KVPages(NamedTuple):
     v_scale: Optional[torch.Tensor] = None
 
 
-def _no_backward(name: str, tensor: torch.Tensor) -> None:
-    if tensor.requires_grad and torch.is_grad_enabled():
+def _no_backward(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
 
 
@@ -299,8 +299,7 @@ def kv_cache_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     """Write the new tokens' keys and values (bf16 ``[tokens, kv_heads, head_dim]``, any row strides that
     are multiples of 8) to their places in the cache, quantising them if the pages are 8-bit.  The pages
     that take new tokens must belong to one sequence each.  Rows of no sequence are ignored."""
-    _no_backward("kv_cache_write", k)
-    _no_backward("kv_cache_write", v)
+    _no_backward("kv_cache_write", k, v, *pages)
     _ext().kv_cache_write(*pages, k, v, block_table, kv_lens, q_starts)
 
 
@@ -310,6 +309,7 @@ def kv_cache_read(pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tens
     """The last tokens of every sequence out of the cache, as ``[total, kv_heads, head_dim]`` keys and
     values (bfloat16 or float32).  ``total`` is the number of rows (``q_starts[-1]``; default: one per
     sequence).  A row before its sequence's first token is zero; rows of no sequence are not written."""
+    _no_backward("kv_cache_read", *pages)
     if total is None:
         if q_starts is not None:
             raise ValueError("kv_cache_read: total (the number of rows) is needed with q_starts")
@@ -331,7 +331,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     a new tensor) must not share memory with ``q``; rows of no sequence are not written.  Whatever lies in
     the pages behind a sequence's end is not looked at; a NaN among the cached tokens of a sequence makes
     its rows NaN."""
-    _no_backward("paged_attention", q)
+    _no_backward("paged_attention", q, out, *pages)
     if max_q_len is None:
         if q_starts is not None:
             raise ValueError("paged_attention: max_q_len is needed with q_starts")
@@ -356,7 +356,7 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     is added; tokens whose bit in ``allowed`` (int32 ``[ceil(vocab / 32)]`` or one row each, token t at bit
     ``t % 32`` of word ``t // 32``) is 0 become ``-inf``.  Computed in fp32.  ``out`` may be ``logits``.
     A token id outside the vocabulary is skipped and recorded (``ops.check_device_errors()``)."""
-    _no_backward("adjust_logits", logits)
+    _no_backward("adjust_logits", logits, repetition_penalty, frequency_penalty, presence_penalty, bias, out)
     return _ext().adjust_logits(logits, out, history, history_lens, prompt_lens, repetition_penalty,
                                 frequency_penalty, presence_penalty, bias, allowed)
 

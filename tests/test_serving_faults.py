@@ -148,3 +148,48 @@ def test_sequences_that_do_not_exist_are_refused(F, seq):
         with pytest.raises(IndexError, match="no sequence"):
             call()
     assert _state(cache) == before
+
+
+@pytest.mark.parametrize("name", ["bias", "repetition_penalty", "frequency_penalty", "presence_penalty", "out"])
+def test_logit_parts_that_want_a_gradient_are_refused(F, name):
+    """There is no backward pass: none is dropped in silence, whichever tensor asks for it."""
+    one = torch.ones(2)
+    args = dict(logits=torch.zeros(2, 40), history=torch.zeros(2, 3, dtype=torch.int64),
+                history_lens=torch.zeros(2, dtype=torch.int32), repetition_penalty=one, frequency_penalty=one,
+                presence_penalty=one, bias=torch.zeros(40), out=torch.zeros(2, 40))
+    args[name] = args[name].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        F.adjust_logits(**args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        F.adjust_logits(**args)
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale", "out"])
+def test_pages_that_want_a_gradient_are_refused(F, name):
+    b = Batch([2, 1], [5, 17], 4, 2, 64, "int8" if "scale" in name else "bf16", 16)
+    pages, out = b.pages(), torch.zeros_like(b.q)
+    if name == "out":
+        out.requires_grad_()
+    else:
+        pages = pages._replace(**{name: getattr(pages, name).clone().requires_grad_()})
+    calls = [lambda: F.paged_attention(b.q, pages, b.table, b.lens, b.starts, b.max_q, out=out)]
+    if name != "out":
+        calls += [lambda: F.kv_cache_write(pages, b.k, b.v, b.table, b.lens, b.starts),
+                  lambda: F.kv_cache_read(pages, b.table, b.lens, b.starts, total=3)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+            call()
+
+
+def test_retract_takes_no_more_than_there_is(F):
+    cache = _cache(_model())
+    cache.extend([0, 1], [17, 3])
+    before = _state(cache)
+    for seqs, rows in (([0, 0], [9, 9]), ([1], [4]), ([0], [-1]), ([0, 1], [1])):
+        with pytest.raises(ValueError, match="retract"):
+            cache.retract(seqs, rows)
+    assert _state(cache) == before
+    cache.retract([0, 1], [2, 3])
+    assert cache.length(0) == 15 and cache.length(1) == 0 and cache.free_pages == 5
