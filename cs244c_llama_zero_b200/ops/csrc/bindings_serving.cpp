@@ -216,8 +216,13 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   c10::DataPtr workspace;
   b200::paged_attention(
       p,
-      [&](size_t bytes) {
-        workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+      [&](size_t bytes, bool can_do_without) -> void* {
+        try {
+          workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+        } catch (const c10::OutOfMemoryError&) {
+          if (!can_do_without) throw;
+          return nullptr;
+        }
         return workspace.get();
       },
       cur_stream());

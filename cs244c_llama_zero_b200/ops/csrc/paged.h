@@ -115,8 +115,8 @@ struct PagedAttnParams {
   DeviceErrors* errs;
 };
 // `alloc` returns device memory of at least the given size (16-byte aligned) that stays valid for the work
-// enqueued on the stream by this call.
-using PagedAlloc = std::function<void*(size_t)>;
+// enqueued on the stream by this call; null where that much is not to be had and the caller can do without.
+using PagedAlloc = std::function<void*(size_t bytes, bool can_do_without)>;
 void paged_attention(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
 // Its form for more than 16 rows per kv head and sequence (paged_chunk.cu).
 void paged_attention_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);

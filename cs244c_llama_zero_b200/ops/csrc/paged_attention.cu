@@ -757,7 +757,7 @@ template <int FMT, int HD, int NT, bool BY_ROWS>
 void launch_decode(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s) {
   using C = DecodeCfg<FMT, HD, NT, BY_ROWS>;
   const int blocks = decode_blocks<FMT, HD, NT, BY_ROWS>();
-  const PagedWorkspace ws = paged_workspace(alloc(paged_workspace_bytes(blocks, C::ROWS, HD)), blocks, C::ROWS);
+  const PagedWorkspace ws = paged_workspace(alloc(paged_workspace_bytes(blocks, C::ROWS, HD), false), blocks, C::ROWS);
   const PagedShape shape{std::max(1, C::ROWS / p.group), kUnitLog2, p.pool.kv_heads};
   launch_k(paged_decode_kernel<FMT, HD, NT, BY_ROWS>, dim3(blocks), dim3(kDecodeThreads), C::SMEM, s, 1, p, shape, ws);
   // one row has many parts when there are few rows, and few when there are many

@@ -1006,7 +1006,8 @@ void launch_attention(const PagedAttnParams& p, const CUtensorMap& tm_q, const C
 // Expanding once pays when rows per kv head and sequence x head_dim reach this (8 int8 caches of 8192 tokens with
 // 8 kv heads, expanded in each tile against once: head_dim 64, 256 rows 73 / 79 us, 512 rows 125 / 117;
 // head_dim 128, 128 rows 104 / 110, 256 rows 151 / 126, 512 rows 250 / 177; 8192 rows over one e4m3 cache of 16384
-// tokens 987 / 560), as long as the units by the block table's width fit this much scratch memory.
+// tokens 987 / 560), as long as the units by the block table's width fit this much scratch memory and the allocator
+// has it.
 constexpr long long kExpandRowColumns = 32768;
 constexpr size_t kExpandBytes = 512u << 20;
 
@@ -1021,7 +1022,7 @@ void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_
   };
   ExpandedUnits ex{};
   if constexpr (FMT == KV_BF16) {
-    const PagedWorkspace ws = paged_workspace(alloc(ws_bytes), blocks, kItemRows);
+    const PagedWorkspace ws = paged_workspace(alloc(ws_bytes, false), blocks, kItemRows);
     const uint64_t rows = (uint64_t)p.seqs.n_pages * p.pool.kv_heads << p.seqs.page_log2;
     launch_attention<FMT, HD>(p, q_map(p.q, p.q_stride_h, p.q_stride_t),
                               make_tmap_bf16_2d(p.pool.k, HD, rows, HD, 64, 1u << p.seqs.page_log2),
@@ -1032,10 +1033,12 @@ void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_
     const size_t kv_bytes = (size_t)unit_blocks * 128 * HD * 2;
     const long long q_rows = (long long)p.seqs.total_q * p.heads;
     const size_t q_bytes = (size_t)q_rows * HD * 2;
-    if ((long long)p.seqs.max_q * p.group * HD >= kExpandRowColumns && unit_blocks > 0 && 2 * kv_bytes <= kExpandBytes) {
-      const size_t power_bytes = ((size_t)unit_blocks * 8 + 255) / 256 * 256;
-      uint8_t* base = reinterpret_cast<uint8_t*>(
-          alloc(ws_bytes + 2 * kv_bytes + power_bytes + (q_bytes + 255) / 256 * 256 + (size_t)q_rows * 4));
+    const size_t power_bytes = ((size_t)unit_blocks * 8 + 255) / 256 * 256;
+    uint8_t* base = nullptr;
+    if ((long long)p.seqs.max_q * p.group * HD >= kExpandRowColumns && unit_blocks > 0 && 2 * kv_bytes <= kExpandBytes)
+      base = reinterpret_cast<uint8_t*>(
+          alloc(ws_bytes + 2 * kv_bytes + power_bytes + (q_bytes + 255) / 256 * 256 + (size_t)q_rows * 4, true));
+    if (base != nullptr) {
       const PagedWorkspace ws = paged_workspace(base, blocks, kItemRows);
       ex.k = reinterpret_cast<__half*>(base + ws_bytes);
       ex.v = ex.k + kv_bytes / 2;
@@ -1052,7 +1055,7 @@ void launch_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_
                                         make_tmap_bf16_2d(ex.k, HD, rows, HD, 64, 128),
                                         make_tmap_bf16_2d(ex.v, HD, rows, HD, 64, 128), shape, ws, ex, s);
     } else {
-      const PagedWorkspace ws = paged_workspace(alloc(ws_bytes), blocks, kItemRows);
+      const PagedWorkspace ws = paged_workspace(alloc(ws_bytes, false), blocks, kItemRows);
       const CUtensorMap none = q_map(p.q, p.q_stride_h, p.q_stride_t);  // nothing is read by TMA
       launch_attention<FMT, HD>(p, none, none, none, shape, ws, ex, s);
     }

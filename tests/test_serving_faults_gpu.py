@@ -126,6 +126,28 @@ def test_values_of_huge_size(F, fmt, heads, q_len, exponent):
     _check(_attend(F, b), b)
 
 
+@pytest.mark.parametrize("fmt", QUANTISED)
+def test_scratch_memory_that_is_not_to_be_had(F, fmt):
+    """Codes are expanded once into scratch memory sized by the block table's width; where the allocator has none left,
+    the same call expands them in its tiles and gives the result all the same."""
+    b = Batch([300], [420], 8, 2, 128, fmt, 128, seed=44)
+    wide = torch.zeros(1, 3000, dtype=torch.int32)  # room for 384000 tokens: 393 MB of fp16 units
+    wide[:, :b.table.shape[1]] = b.table
+    args = (b.q.cuda(), b.pages("cuda"), wide.cuda(), b.lens.cuda(), b.starts.cuda(), b.max_q)
+    roomy = F.paged_attention(*args)
+    _check(roomy, b)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (100 << 20)) / total)
+        out = F.paged_attention(*args)
+        torch.cuda.synchronize()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    _check(out, b)
+
+
 # ------------------------------------------------------------------------------------------ precision
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("heads,q_len", FORMS + [((12, 4, 64), 1), ((32, 8, 128), 1), ((12, 4, 64), 400), ((32, 8, 64), 90)])
