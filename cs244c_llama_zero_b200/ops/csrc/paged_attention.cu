@@ -414,11 +414,14 @@ __global__ void __launch_bounds__(kDecodeThreads)
       if constexpr (QUANT) {
         const uint32_t sa = tile + 2 * C::TILE + n * 4;
         const float k0 = lds32f(sa), k1 = lds32f(sa + 32), v0 = lds32f(sa + 64), v1 = lds32f(sa + 96);
-        // a scale of 0 (all codes 0) counts as 2^kLowestExponent, one below 2^-100 as that; a NaN stays one
-        const float x0 = lg2_approx(v0 == 0.f ? kZeroScale : fmaxf(v0, 7.888609e-31f)) + (v0 - v0);
-        const float x1 = lg2_approx(v1 == 0.f ? kZeroScale : fmaxf(v1, 7.888609e-31f)) + (v1 - v1);
+        // a scale of 0 (all codes 0) counts as 2^kLowestExponent, one below 2^-100 as that; one that is no number
+        // goes into the scores alone: rows that do not see the token add 0 * w
+        float x0 = lg2_approx(v0 == 0.f ? kZeroScale : fmaxf(v0, 7.888609e-31f));
+        float x1 = lg2_approx(v1 == 0.f ? kZeroScale : fmaxf(v1, 7.888609e-31f));
         w0 = ex2_approx(-x0);
         w1 = ex2_approx(-x1);
+        x0 += v0 - v0;
+        x1 += v1 - v1;
 #pragma unroll
         for (int t = 0; t < N; ++t) {
           s[t][0] = fmaf(s[t][0], k0 * q_unit[t][0], x0);

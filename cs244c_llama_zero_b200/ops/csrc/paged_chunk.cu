@@ -155,11 +155,22 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 // 2^e, and the exponent e that brings max_code * scale into (2^14, 2^15] (the lowest one for a scale of 0).
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ int unit_exponent(uint32_t scale_bits, float max_code) {
-  if (scale_bits == 0u) return kLowestExponent;
-  const int e = (int)(__float_as_uint(__uint_as_float(scale_bits) * max_code) >> 23) - 127;  // floor(log2)
+__device__ __forceinline__ int unit_exponent(uint32_t top, float max_code) {
+  if (top == 0u) return kLowestExponent;
+  const int e = (int)(__float_as_uint(__uint_as_float(top) * max_code) >> 23) - 127;  // floor(log2)
   return max(e - 14, kLowestExponent);  // (113 for the largest bf16 values)
 }
+
+// A token whose V has no finite scale is lost to the rows that see it, and has to be nothing to the others, although
+// a probability of 0 times a NaN is NaN: its V becomes zeros and its K NaN, since masked scores are replaced.
+__device__ __forceinline__ void settle_scales(float& k, float& v) {
+  if (v - v != 0.f) {
+    k = __int_as_float(0x7FC00000);
+    v = 0.f;
+  }
+}
+// What a scale counts as in its unit's maximum: scales are not negative; infinities and NaN do not count.
+__device__ __forceinline__ uint32_t scale_bits(float x) { return x - x == 0.f ? __float_as_uint(x) : 0u; }
 
 template <int FMT>
 __device__ __forceinline__ void expand16(const uint4& q, float factor, uint4 (&out)[2]) {
@@ -523,6 +534,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
                         ((j * 128 + tid) & ((1 << page_log2) - 1));
           k_scale = p.pool.k_scale[c];
           v_scale = p.pool.v_scale[c];
+          settle_scales(k_scale, v_scale);
         }
       };
       // Q: a thread takes a row of each tile
@@ -582,9 +594,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         // the unit's powers of two
         scales[g & 1][0][tid] = k_scale;
         scales[g & 1][1][tid] = v_scale;
-        // scales are not negative; a NaN does not count here
-        uint32_t km = __reduce_max_sync(0xffffffffu, k_scale == k_scale ? __float_as_uint(k_scale) : 0u);
-        uint32_t vm = __reduce_max_sync(0xffffffffu, v_scale == v_scale ? __float_as_uint(v_scale) : 0u);
+        uint32_t km = __reduce_max_sync(0xffffffffu, scale_bits(k_scale));
+        uint32_t vm = __reduce_max_sync(0xffffffffu, scale_bits(v_scale));
         if (lane == 0) maxima[g & 1][warp & 3] = make_uint2(km, vm);
         named_bar(1, 128);
 #pragma unroll
@@ -941,13 +952,13 @@ __global__ void __launch_bounds__(128) paged_expand_kernel(PagedAttnParams p, Ex
     else
       report_error(p.errs, kErrBadIndex, b);
   }
-  const float ks = cell >= 0 ? p.pool.k_scale[cell] : 0.f, vs = cell >= 0 ? p.pool.v_scale[cell] : 0.f;
+  float ks = cell >= 0 ? p.pool.k_scale[cell] : 0.f, vs = cell >= 0 ? p.pool.v_scale[cell] : 0.f;
+  settle_scales(ks, vs);
   cells[tid] = cell;
   scales[0][tid] = ks;
   scales[1][tid] = vs;
-  // scales are not negative; a NaN does not count here
-  uint32_t km = __reduce_max_sync(0xffffffffu, ks == ks ? __float_as_uint(ks) : 0u);
-  uint32_t vm = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
+  uint32_t km = __reduce_max_sync(0xffffffffu, scale_bits(ks));
+  uint32_t vm = __reduce_max_sync(0xffffffffu, scale_bits(vs));
   if (lane == 0) maxima[tid >> 5] = make_uint2(km, vm);
   __syncthreads();
 #pragma unroll

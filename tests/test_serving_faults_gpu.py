@@ -127,6 +127,29 @@ def test_values_of_huge_size(F, fmt, heads, q_len, exponent):
 
 
 @pytest.mark.parametrize("fmt", QUANTISED)
+@pytest.mark.parametrize("heads,q_len", FORMS + [((4, 4, 64), 130), ((4, 4, 128), 300), ((64, 1, 64), 5)])
+@pytest.mark.parametrize("bad", ["k nan", "v nan", "v inf", "v -inf"])
+def test_poisoned_tokens_in_masked_places(F, fmt, heads, q_len, bad):
+    """A NaN or an infinity in a new token's key or value: the rows ahead of it do not see it and are what they are
+    without it; the rows from it on are NaN."""
+    b = Batch([q_len, q_len], [q_len + 75, q_len + 9], *heads, fmt, 16, seed=43)
+    want = b.attention()
+    kv, hd = heads[1], heads[2]
+    new = q_len // 2  # the poisoned row of sequence 0
+    pos = b.kv_lens[0] - q_len + new
+    pages = b.pages("cuda")
+    k, v = torch.ones(1, kv, hd), torch.ones(1, kv, hd)
+    (k if bad[0] == "k" else v)[0, :, 5] = float(bad[2:])
+    at = torch.tensor([pos + 1], dtype=torch.int32).cuda()
+    F.kv_cache_write(pages, k.bfloat16().cuda(), v.bfloat16().cuda(), b.table[:1].cuda(), at)
+    out = F.paged_attention(b.q.cuda(), pages, b.table.cuda(), b.lens.cuda(), b.starts.cuda(), b.max_q)
+    _check(out, b, want, rows=slice(0, new))
+    _check(out, b, want, rows=slice(q_len, 2 * q_len))
+    seen = out[new:q_len].float().cpu()
+    assert torch.isnan(seen).all()
+
+
+@pytest.mark.parametrize("fmt", QUANTISED)
 def test_scratch_memory_that_is_not_to_be_had(F, fmt):
     """Codes are expanded once into scratch memory sized by the block table's width; where the allocator has none left,
     the same call expands them in its tiles and gives the result all the same."""
