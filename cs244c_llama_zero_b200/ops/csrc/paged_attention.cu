@@ -487,12 +487,47 @@ __global__ void __launch_bounds__(kDecodeThreads)
         pf[t][1] = transpose_8x8(pack_pair<QUANT>(p2, p3));
       }
       if constexpr (!QUANT) {
+        // Where some rows do not see all tokens, infinities and NaN are taken out of V (0 times them would be NaN)
+        // and put back as NaN into the columns of the rows that do see them.
+        if (t0 + 16 > all_see && rows > p.group) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          uint32_t a[4];
-          ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
+          for (int i = 0; i < KS; ++i) {
+            uint32_t a[4], bad[4];
+            ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
 #pragma unroll
-          for (int t = 0; t < N; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
+            for (int x = 0; x < 4; ++x) {
+              bad[x] = __vcmpeq2(a[x] & 0x7F807F80u, 0x7F807F80u);
+              a[x] &= ~bad[x];
+            }
+#pragma unroll
+            for (int t = 0; t < N; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
+            if (!__any_sync(0xffffffffu, (bad[0] | bad[1] | bad[2] | bad[3]) != 0u)) continue;
+            // columns 16 i + n (a[0], a[2]) and 8 more (a[1], a[3]); tokens 2 j, 2 j + 1 and 8 more
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              int lowest = 16;  // token that holds one
+#pragma unroll
+              for (int x = 3; x >= 0; --x)
+                if ((bad[h + (x & 2)] >> (16 * (x & 1))) & 1u) lowest = 2 * j + 4 * (x & 2) + (x & 1);
+              lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 1));
+              lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 2));
+#pragma unroll
+              for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int lim = min(base_pos + (row0 + t * row_step + 2 * j + e) / p.group + 1, visible);
+                  if (lowest < 16 && t0 + lowest < lim) o[i][t][2 * h + e] = __int_as_float(0x7FC00000);
+                }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            uint32_t a[4];
+            ldsm_x4_t((va ^ (((2 * i) & 7) << 4)) + (i >> 2) * 128, a);
+#pragma unroll
+            for (int t = 0; t < N; ++t) mma_16816<false>(o[i][t], a, pf[t][0], pf[t][1]);
+          }
         }
       } else {
         // tile i: O's rows n and n + 8 are columns n * HD / 8 + 2 i and + 1 of V; words of tokens
