@@ -7,7 +7,8 @@
 //
 // Warpgroups (the first hands registers to the others with setmaxnreg):
 //   0: warp 0 loads Q (TMA: box of 64 columns x group heads x tokens) and, for bf16 pages, K and V (TMA: one box
-//      per page and 64 columns); warp 1 issues the MMAs; warp 2 zeroes V's rows behind the last visible token.
+//      per page and 64 columns); warp 1 issues the MMAs; warps 2 and 3 go through V of the units that not all rows
+//      see whole.
 //   1, 2: softmax of tile A and B, one thread per row, as in the training forward kernel: scores from tensor
 //      memory, probabilities back into the same columns as the A operand of the PV product, lazy rescaling of O.
 //   3 (8-bit pages only): loads Q, and expands codes into the shared-memory tiles; see below.
@@ -23,9 +24,11 @@
 // powers of two beside them, and Q's rows, and the attention kernel loads both by TMA (KV_EXPANDED).
 // MMA order: S_A(0) S_B(0) | PV_A(j) S_A(j+1) PV_B(j) S_B(j+1) | ...
 //
-// Masking is by selection (a masked score becomes -inf whatever K holds), and V's rows behind the last visible
-// token are zeroed in shared memory before they meet the zero probabilities: what lies in a page behind a
-// sequence's end, a NaN included, has no influence.
+// Masking is by selection (a masked score becomes -inf whatever K holds).  A probability of 0 times an infinity or a NaN
+// is NaN, so V must hold none where some row of an item does not see it.  V's rows behind the last visible token
+// are zeroed in shared memory: what lies in a page behind a sequence's end has no influence.  Infinities and NaN ahead
+// of it, in units that not all rows see whole, are zeroed too (bf16); a block that met some looks them up in the cache
+// once more in its epilogue, and writes NaN into the columns that held them for the rows that see them.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -88,7 +91,7 @@ struct ChunkCfg {
   static constexpr int BAR_OFF = KV_OFF + STAGES * STAGE_BYTES;
   static constexpr int UNIT_OFF = BAR_OFF + 256;  // 8-bit: powers of two of Q's rows, K's and V's units
   static constexpr int SMEM_BYTES = UNIT_OFF + (QUANT ? Q_BUFS * 1024 + 128 : 0) + 1024;
-  static_assert(SMEM_BYTES + 2048 <= 232448, "shared memory exceeds 227 KB");
+  static_assert(SMEM_BYTES + 4096 <= 232448, "shared memory exceeds 227 KB");
   static constexpr int TMEM_COLS = 512;
   static constexpr int T_S = 0;
   static constexpr int T_O = 256;
@@ -103,13 +106,17 @@ struct ChunkWalk {
   int j0, j1;      // units of the item in it
   int n_tiles;     // 1: the item has rows in tile A only
   int visible;     // cached tokens that its last row sees
+  int all_see;     // and its first row (may be negative)
 };
 __device__ __forceinline__ void enter_item(ChunkWalk& w, const PagedShape& sh, int j0) {
   w.j0 = j0;
   w.j1 = unit_of_cut(w.it, w.end);
   w.n_tiles = w.it.seq.qn - w.it.rt * sh.tile_tokens > sh.tile_tokens / 2 ? 2 : 1;
   w.visible = item_visible(w.it.seq, w.it.rt, sh.tile_tokens);
+  w.all_see = w.it.seq.len - w.it.seq.qn + w.it.rt * sh.tile_tokens + 1;
 }
+// The unit from which on some row of the item does not see all 128 tokens.
+__device__ __forceinline__ int first_hidden_unit(const ChunkWalk& w) { return max(w.all_see, 0) >> 7; }
 // By one thread.  False at the end of the range.
 __device__ __forceinline__ bool next_part(ChunkWalk& w, const PagedSeqs& s, const PagedShape& sh) {
   if (w.end <= item_end(w.it)) return false;
@@ -227,6 +234,46 @@ __device__ __forceinline__ void mask32(uint32_t (&s)[32], int seen) {
   }
 }
 
+// By two warps (`half` 0 and 1), each on its half of the 16-byte pieces: takes infinities and NaN out of the first
+// `live` rows of a V tile (128 rows, 64 columns per 16 KB block); true if there were any.  x * 0 is NaN for those and
+// for nothing else: one instruction for two values finds whether there are any, and most tiles have none.
+template <int HD>
+__device__ __forceinline__ bool take_out_non_finite(uint8_t* vs, int live, int half, int lane) {
+  const int first = half * 32 + lane;
+  uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int kb = 0; kb < HD / 64; ++kb)
+#pragma unroll 8
+    for (int i = first; i < live * 8; i += 64) {
+      const uint4 x = *reinterpret_cast<const uint4*>(vs + kb * 16384 + i * 16);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc[e]) : "r"(w[e]), "r"(0u));
+    }
+  if (!__any_sync(0xffffffffu, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7FFF7FFFu) != 0u)) return false;
+  for (int kb = 0; kb < HD / 64; ++kb)
+    for (int i = first; i < live * 8; i += 64) {
+      uint16_t* piece = reinterpret_cast<uint16_t*>(vs + kb * 16384 + i * 16);
+      for (int e = 0; e < 8; ++e)
+        if ((piece[e] & 0x7F80) == 0x7F80) piece[e] = 0;
+    }
+  return true;
+}
+// By a row's thread, in the rare block that took some out: NaN into the columns in which the tokens t0 to t1 that the
+// row sees hold one, behind what the thread has written there.  put(d) writes column d.
+template <typename Put>
+__device__ __forceinline__ void put_back_nan(const PagedAttnParams& p, int b, int kvh, int t0, int t1, const Put& put) {
+  const int page_log2 = p.seqs.page_log2, hd = p.pool.head_dim;
+  for (int t = t0; t < t1; ++t) {
+    const int page = p.seqs.table[(long long)b * p.seqs.table_stride + (t >> page_log2)];
+    if (page < 0 || page >= p.seqs.n_pages) continue;
+    const long long cell = (((long long)page * p.pool.kv_heads + kvh) << page_log2) + (t & ((1 << page_log2) - 1));
+    const uint16_t* v = reinterpret_cast<const uint16_t*>(p.pool.v) + cell * hd;
+    for (int d = 0; d < hd; ++d)
+      if ((v[d] & 0x7F80) == 0x7F80) put(d);
+  }
+}
+
 template <int FMT, int HD>
 __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -244,10 +291,12 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
   uint64_t* p_full = s_full + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* o_free = o_done + 2;
-  uint64_t* v_zeroed = o_free + 2;  // per stage (bf16): V's rows behind the last visible token are zeros
-  uint64_t* v_raw = v_zeroed + C::STAGES;  // per stage (bf16): V of such a tile has arrived
+  // bf16, per stage, of units that some row does not see whole: V has arrived (v_raw), is fit for the product (v_clean)
+  uint64_t* v_clean = o_free + 2;
+  uint64_t* v_raw = v_clean + C::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_raw + C::STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* taken_out = abort_flag + 1;  // bf16: some V of this block held an infinity or a NaN
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -258,7 +307,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&kv_full[s], C::QUANT ? 4 : 1);
       mbar_init(&kv_empty[s], 1);
-      mbar_init(&v_zeroed[s], 1);
+      mbar_init(&v_clean[s], 2);
       mbar_init(&v_raw[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -268,6 +317,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
       mbar_init(&o_free[t], 4);
     }
     *abort_flag = 0;
+    *taken_out = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -329,6 +379,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         {
           const int* table = p.seqs.table + (long long)w.it.b * p.seqs.table_stride;
           const int page_size = 1 << page_log2, kvh = w.it.kvh, visible = w.visible, j1 = w.j1;
+          const int hidden = first_hidden_unit(w);
           for (int j = w.j0; j < j1; ++j, ++g) {
             const int st = g % C::STAGES;
             if (!mbar_wait_bounded(&kv_empty[st], ((g / C::STAGES) & 1) ^ 1u, abort_flag, p.errs, kErrAttnWait, 0)) {
@@ -348,12 +399,11 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
               continue;
             }
             const int n_pages = min(128 >> page_log2, max(0, (visible - j * 128 + page_size - 1) >> page_log2));
-            // a tile that the sequence ends in gets V on a barrier of its own: warp 2 zeroes its tail first
-            const bool tail = (j + 1) * 128 > visible;
-            uint64_t* v_bar = tail ? &v_raw[st] : &kv_full[st];
+            // a unit that is not seen whole gets V on a barrier of its own: warps 2 and 3 go through it first
+            uint64_t* v_bar = j >= hidden ? &v_raw[st] : &kv_full[st];
             const int bytes = n_pages * page_size * HD * 2;
-            mbar_expect_tx(&kv_full[st], tail ? bytes : 2 * bytes);
-            if (tail) mbar_expect_tx(&v_raw[st], bytes);
+            mbar_expect_tx(&kv_full[st], j >= hidden ? bytes : 2 * bytes);
+            if (j >= hidden) mbar_expect_tx(&v_raw[st], bytes);
             for (int i = 0; i < n_pages; ++i) {
               int page = table[((j * 128) >> page_log2) + i];
               if (page < 0 || page >= p.seqs.n_pages) {
@@ -379,7 +429,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 128, false, false) ^ F16;
       constexpr uint32_t IDESC_O = idesc_bf16_f32(128, C::O_COLS, false, true) ^ F16;
       int g = 0;
-      uint32_t zeroed_parity = 0;  // bit per stage
+      uint32_t clean_parity = 0;  // bit per stage
       int pn[2] = {0, 0}, on[2] = {0, 0};
       bool ok = true;
       for (int k = 0; ok; ++k) {
@@ -396,7 +446,7 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           }
           tc_commit(&s_full[t]);
         };
-        const int j0 = w.j0, n = w.j1 - j0, n_tiles = w.n_tiles, visible = w.visible;
+        const int j0 = w.j0, n = w.j1 - j0, n_tiles = w.n_tiles, hidden = first_hidden_unit(w);
         int st = g % C::STAGES;
         if (!mbar_wait_bounded(&kv_full[st], (g / C::STAGES) & 1, abort_flag, p.errs, kErrAttnWait, 1)) break;
         tc_fence_after();
@@ -405,12 +455,12 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           st = (g + j) % C::STAGES;
           const int st1 = (g + j + 1) % C::STAGES;
           if constexpr (!C::F16) {
-            if ((j0 + j + 1) * 128 > visible) {
-              if (!mbar_wait_bounded(&v_zeroed[st], (zeroed_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 7)) {
+            if (j0 + j >= hidden) {
+              if (!mbar_wait_bounded(&v_clean[st], (clean_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 7)) {
                 ok = false;
                 break;
               }
-              zeroed_parity ^= 1u << st;
+              clean_parity ^= 1u << st;
             }
           }
           bool next_loaded = false;
@@ -457,28 +507,32 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         tc_commit(&q_empty[qs]);
         if (!ok || !next_part(w, p.seqs, shape)) break;
       }
-    } else if (!C::F16 && busy && warp == 2) {
+    } else if (!C::F16 && busy && warp >= 2) {
+      const int half = warp - 2;
       int g = 0;
       uint32_t raw_parity = 0;  // bit per stage
       while (true) {
-        g += w.j1 - w.j0;
-        const int live = w.visible - (w.j1 - 1) * 128;  // only an item's last tile can have a tail
-        if (live < 128) {
-          const int st = (g - 1) % C::STAGES;
-          const bool ok =
-              mbar_wait_bounded(&v_raw[st], (raw_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 8);
-          if (!__all_sync(0xffffffffu, ok)) break;
+        bool ok = true;
+        for (int j = max(w.j0, first_hidden_unit(w)); j < w.j1; ++j) {
+          const int st = (g + j - w.j0) % C::STAGES;
+          ok = mbar_wait_bounded(&v_raw[st], (raw_parity >> st) & 1, abort_flag, p.errs, kErrAttnWait, 8);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           raw_parity ^= 1u << st;
           uint8_t* vs = smem + C::KV_OFF + st * C::STAGE_BYTES + C::TILE_BYTES;
-          const int dead = 128 - max(live, 0);
+          const int live = min(max(w.visible - j * 128, 0), 128);
 #pragma unroll
           for (int kb = 0; kb < C::KB; ++kb)
-            for (int i = lane; i < dead * 8; i += 32)
-              *reinterpret_cast<uint4*>(vs + kb * 16384 + (128 - dead) * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = live * 8 + half * 32 + lane; i < 1024; i += 64)
+              *reinterpret_cast<uint4*>(vs + kb * 16384 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          if (w.all_see < w.visible)  // (else all rows are of one token and see the same)
+            if (take_out_non_finite<HD>(vs, live, half, lane) && lane == 0) *taken_out = 1;
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&v_zeroed[st]);
+          if (lane == 0) mbar_arrive(&v_clean[st]);
         }
+        if (!ok) break;
+        g += w.j1 - w.j0;
         if (!next_part_warp(w, p.seqs, shape, lane)) break;
       }
     }
@@ -838,6 +892,15 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
           }
         }
         if (!whole && live) ws.ml[(size_t)slot * kItemRows + row] = make_float2(m_used, l);
+        if constexpr (!C::F16) {
+          if (*taken_out != 0 && live && w.all_see < w.visible)
+            put_back_nan(p, w.it.b, w.it.kvh, max(j0, first_hidden_unit(w)) * 128, min(lim, j1 * 128), [&](int d) {
+              if (whole)
+                reinterpret_cast<uint16_t*>(dst)[d] = 0x7FC0;
+              else
+                reinterpret_cast<float*>(part + (size_t)(d / 4) * kItemRows)[d % 4] = __int_as_float(0x7FC00000);
+            });
+        }
       }
       g += j1 - j0;
       if (!next_part_warp(w, p.seqs, shape, lane)) break;

@@ -325,12 +325,12 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     Row i of a sequence's q_len new tokens stands at position ``kv_len - q_len + i`` and sees the cached
     tokens up to and including that position (their keys and values must have been written); a row whose
     position is negative sees nothing and gives zeros.  Query head h reads kv head
-    ``h // (heads / kv_heads)``; scores are scaled by ``scale`` (default ``head_dim ** -0.5``;
-    2^-126 to 1e30).
+    ``h // (heads / kv_heads)``; scores are scaled by ``scale`` (2^-126 to 1e30; default ``head_dim ** -0.5``).
     ``max_q_len`` bounds the new tokens of any sequence and is required with ``q_starts``.  ``out`` (default:
-    a new tensor) must not share memory with ``q``; rows of no sequence are not written.  Whatever lies in
-    the pages behind a sequence's end is not looked at; a NaN among the cached tokens of a sequence makes
-    its rows NaN."""
+    a new tensor) must not share memory with ``q``; rows of no sequence are not written.  What a row does not
+    see has no influence on it, whatever it is: tokens behind its position, the pages behind a sequence's end.
+    An infinity or a NaN in a key that it does see makes it NaN, one in a value too (8-bit pages) or its column
+    not finite (bf16)."""
     _no_backward("paged_attention", q, out, *pages)
     if max_q_len is None:
         if q_starts is not None:
