@@ -193,3 +193,31 @@ def test_retract_takes_no_more_than_there_is(F):
     assert _state(cache) == before
     cache.retract([0, 1], [2, 3])
     assert cache.length(0) == 15 and cache.length(1) == 0 and cache.free_pages == 5
+
+
+# ------------------------------------------------------------------------------------------ generation without a cache
+def _generate_by_concatenation(model, ids, count, temperature, top_k):
+    """Generation by appending each token to a tensor of its own."""
+    with torch.no_grad():
+        for _ in range(count):
+            last = model(ids[:, -model.cfg.max_seq_len:]).logits[:, -1]
+            ids = torch.cat([ids, model._pick_next(last, temperature, top_k)], dim=1)
+    return ids
+
+
+@pytest.mark.parametrize("prompt", [1, 7, 16, 23])
+@pytest.mark.parametrize("temperature,top_k", [(0.0, None), (1.0, None), (0.7, 5)])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_generation_without_a_cache(prompt, temperature, top_k, dtype):
+    """Several sequences, prompts shorter and longer than the window, and past its end."""
+    from cs244c_llama_zero_b200.models import LlamaForCausalLM, ModelConfig
+
+    torch.manual_seed(1)
+    model = LlamaForCausalLM(ModelConfig(name="t", vocab_size=97, max_seq_len=16, dim=64, n_layers=2, n_heads=4,
+                                         n_kv_heads=2, ffn_dim=64, initializer_range=0.2)).eval()
+    ids = torch.randint(0, 97, (3, prompt), dtype=dtype)
+    torch.manual_seed(2)
+    want = _generate_by_concatenation(model, ids, 20, temperature, top_k)
+    torch.manual_seed(2)
+    got = model.generate(ids, 20, temperature=temperature, top_k=top_k)
+    assert got.dtype == want.dtype and torch.equal(got, want)

@@ -204,3 +204,35 @@ def test_scales_of_different_size_in_a_unit(F, fmt, heads, q_len):
     b.scales[0][:, :, ::7] *= 2.0 ** -12
     b.scales[1][:, :, ::7] *= 2.0 ** 12
     _check(_attend(F, b), b)
+
+
+# ------------------------------------------------------------------------------------------ generation
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("fmt", list(FORMATS))
+def test_the_next_token_with_and_without_a_cache(hd, fmt):
+    """The same backend with a cache and without one picks the same token wherever the 64-bit model's two best
+    logits are further apart than what both paths' logits are off by."""
+    from cs244c_llama_zero_b200.models import LlamaForCausalLM, ModelConfig, PagedKVCache
+
+    cfg = ModelConfig(name="gen", vocab_size=1000, max_seq_len=140, dim=4 * hd, n_layers=3, n_heads=4, n_kv_heads=2,
+                      ffn_dim=512, initializer_range=0.08)
+    torch.manual_seed(3)
+    model = LlamaForCausalLM(cfg).cuda().to(torch.bfloat16).eval()
+    oracle = LlamaForCausalLM(cfg).cuda().double().eval()
+    oracle.load_state_dict({k: v.double() for k, v in model.state_dict().items()})
+    model.set_backend("b200")
+    ids = torch.randint(0, cfg.vocab_size, (24, 128), device="cuda")
+    with torch.no_grad():
+        want = oracle(ids).logits[:, -1]
+        plain = model(ids).logits[:, -1].double()
+        cache = PagedKVCache.for_batch(cfg, 24, 128, dtype=fmt)
+        cached = model.decode_step(ids.reshape(-1), cache, range(24), [128] * 24).double()
+        off = torch.maximum((plain - want).abs().amax(-1), (cached - want).abs().amax(-1))
+        best = want.topk(2, dim=-1).values
+        clear = best[:, 0] - best[:, 1] > 2 * off  # either of the two logits may be off by that much
+        assert clear.any()
+        with_cache = model.generate(ids, 1, temperature=0.0, kv_cache=fmt)
+        without = model.generate(ids, 1, temperature=0.0)
+    assert torch.equal(with_cache[:, :128], ids) and torch.equal(without[:, :128], ids)
+    assert torch.equal(with_cache[clear, 128], without[clear, 128])
+    assert torch.equal(without[clear, 128], want.argmax(-1)[clear])
