@@ -110,7 +110,9 @@ __global__ void __launch_bounds__(kThreads)
       const long long place = __shfl_sync(0xffffffffu, run.place, tok & 31);
       const int h = pass * HEADS + lane / LANES;
       cell[i] = -1;
-      if (i0 + i < total && place >= 0 && h < pool.kv_heads) {
+      if (i0 + i < total && place >= 0 && h < pool.kv_heads &&
+          B200_IN_BOUNDS(errs, run.t0 + tok, 1, seqs.total_q, 130) &&
+          B200_IN_BOUNDS(errs, place + (h << seqs.page_log2), 1, pool_cells(seqs, pool.kv_heads), 131)) {
         cell[i] = place + (h << seqs.page_log2);
         x[i] = *reinterpret_cast<const uint4*>(from);
       }
@@ -197,10 +199,11 @@ __global__ void __launch_bounds__(kThreads)
       at[i] = -1;
       const long long place = __shfl_sync(0xffffffffu, run.place, tok & 31);
       const int h = pass * HEADS + lane / LANES;
-      if (i0 + i < total && place != kNoSequence && h < pool.kv_heads) {
+      if (i0 + i < total && place != kNoSequence && h < pool.kv_heads &&
+          B200_IN_BOUNDS(errs, run.t0 + tok, 1, seqs.total_q, 132)) {
         at[i] = ((long long)(run.t0 + tok) * pool.kv_heads + h) * HD + sub * 8;
-        if (place >= 0) {
-          const long long cell = place + ((long long)h << seqs.page_log2);
+        const long long cell = place + ((long long)h << seqs.page_log2);
+        if (place >= 0 && B200_IN_BOUNDS(errs, cell, 1, pool_cells(seqs, pool.kv_heads), 133)) {
           if constexpr (FMT == KV_BF16) {
             x[i] = *reinterpret_cast<const uint4*>(src + cell * (2 * HD) + sub * 16);
           } else {

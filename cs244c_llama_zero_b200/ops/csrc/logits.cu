@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, MIN_BLOCKS) adjust_logits_kernel(Log
         return false;
       }
       const int at = (int)t - base;
-      if (at < 0 || at >= RANGE) return false;
+      if (at < 0 || at >= RANGE || !B200_IN_BOUNDS(p.errs, place, 1, p.max_history, 153)) return false;
       if (place >= prompt) atomicAdd(&counts[at], 1u);
       return ((atomicOr(&seen[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1u) == 0u;
     };
@@ -181,10 +181,11 @@ __global__ void __launch_bounds__(kThreads, MIN_BLOCKS) adjust_logits_kernel(Log
           Vec<T> y = *reinterpret_cast<const Vec<T>*>(src + t0);
 #pragma unroll
           for (int e = 0; e < VE; ++e) y.e[e] = adjusted(to_f32(y.e[e]), t0 + e);
-          *reinterpret_cast<Vec<T>*>(dst + t0) = y;
+          if (B200_IN_BOUNDS(p.errs, t0, VE, p.vocab, 151)) *reinterpret_cast<Vec<T>*>(dst + t0) = y;
         } else {
 #pragma unroll 1
-          for (int t = max(t0, 0); t < min(t0 + VE, p.vocab); ++t) dst[t] = adjusted(to_f32(src[t]), t);
+          for (int t = max(t0, 0); t < min(t0 + VE, p.vocab); ++t)
+            if (B200_IN_BOUNDS(p.errs, t, 1, p.vocab, 152)) dst[t] = adjusted(to_f32(src[t]), t);
         }
       }
       continue;
@@ -235,7 +236,8 @@ __global__ void __launch_bounds__(kThreads, MIN_BLOCKS) adjust_logits_kernel(Log
       Vec<T> y;
 #pragma unroll
       for (int e = 0; e < VE; ++e) y.e[e] = from_f32<T>(l[e]);
-      *reinterpret_cast<Vec<T>*>(out + i * GROUPS) = y;
+      if (B200_IN_BOUNDS(p.errs, at + tid * VE + i * GROUPS, VE, p.vocab, 150))
+        *reinterpret_cast<Vec<T>*>(out + i * GROUPS) = y;
     }
   }
 }

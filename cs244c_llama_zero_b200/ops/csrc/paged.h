@@ -32,6 +32,11 @@ struct PagedSeqs {
   int max_q;    // bound on a sequence's new tokens
 };
 
+// Rows of a pool: (page, head, offset) cells.
+__host__ __device__ inline long long pool_cells(const PagedSeqs& s, int kv_heads) {
+  return (long long)s.n_pages * kv_heads << s.page_log2;
+}
+
 struct SeqInfo {
   int q0, qn, len;
   bool ok;

@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
         if (lane == 0) report_error(p.errs, kErrBadIndex, li.b);
         live = 0;
       }
-      const long long cell =
-          live > 0 ? (((long long)page * shape.kv_heads + li.kvh) << page_log2) + (t0 & page_mask) : 0;
+      long long cell = live > 0 ? (((long long)page * shape.kv_heads + li.kvh) << page_log2) + (t0 & page_mask) : 0;
+      if (!B200_IN_BOUNDS(p.errs, cell, max(live, 1), pool_cells(p.seqs, shape.kv_heads), 135)) cell = live = 0;
       const uint8_t* k_src = reinterpret_cast<const uint8_t*>(p.pool.k) + cell * C::ROW_BYTES + lane * 16;
       const uint8_t* v_src = reinterpret_cast<const uint8_t*>(p.pool.v) + cell * C::ROW_BYTES + lane * 16;
       const uint32_t k_dst = slot_in + k_off0, v_dst = slot_in + v_off0;
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = row0 + t * row_step + n;
-      const bool ok = r < rows;
+      const bool ok = r < rows && B200_IN_BOUNDS(p.errs, x.seq.q0 + tok0 + r / p.group, 1, p.seqs.total_q, 134);
       const __nv_bfloat16* src = p.q + (long long)(x.seq.q0 + tok0 + r / p.group) * p.q_stride_t +
                                  (long long)(x.kvh * p.group + r % p.group) * p.q_stride_h;
       if constexpr (!QUANT) {
@@ -644,11 +644,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
         a.w += v.w;
       }
       if (whole) {
+        if (!B200_IN_BOUNDS(p.errs, q0 + r / p.group, 1, p.seqs.total_q, 136)) continue;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         __nv_bfloat16* dst = p.out + (long long)(q0 + r / p.group) * p.o_stride_t +
                              (long long)(head0 + r % p.group) * p.o_stride_h + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
-      } else {
+      } else if (B200_IN_BOUNDS(p.errs, (long long)slot * C::ROWS + r, 1, 2ll * gridDim.x * C::ROWS, 137)) {
         *reinterpret_cast<float4*>(ws.o + ((size_t)slot * C::ROWS + r) * HD + d) = a;
         if (d == 0) ws.ml[(size_t)slot * C::ROWS + r] = make_float2(mx, sum);
       }
@@ -757,7 +758,7 @@ __global__ void __launch_bounds__(kJoinThreads)
         }
       __syncthreads();
     }
-    if (live && sub == 0) {
+    if (live && sub == 0 && B200_IN_BOUNDS(p.errs, seq.q0 + tok0 + r / p.group, 1, p.seqs.total_q, 138)) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = p.out + (long long)(seq.q0 + tok0 + r / p.group) * p.o_stride_t +
                            (long long)(rec.kvh * p.group + r % p.group) * p.o_stride_h + lane * V;

@@ -578,7 +578,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           q[v][i] = make_uint4(0u, 0u, 0u, 0u);
-          if (cell[i] >= 0) q[v][i] = *reinterpret_cast<const uint4*>(src + (long long)cell[i] * HD);
+          if (cell[i] >= 0 && B200_IN_BOUNDS(p.errs, cell[i], 1, pool_cells(p.seqs, shape.kv_heads), 141))
+            q[v][i] = *reinterpret_cast<const uint4*>(src + (long long)cell[i] * HD);
         }
       };
       auto load_scales = [&]() {
@@ -586,8 +587,10 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         if (next_scale_page >= 0 && next_scale_page < p.seqs.n_pages) {
           const int c = ((next_scale_page * shape.kv_heads + w.it.kvh) << page_log2) +
                         ((j * 128 + tid) & ((1 << page_log2) - 1));
-          k_scale = p.pool.k_scale[c];
-          v_scale = p.pool.v_scale[c];
+          if (B200_IN_BOUNDS(p.errs, c, 1, pool_cells(p.seqs, shape.kv_heads), 142)) {
+            k_scale = p.pool.k_scale[c];
+            v_scale = p.pool.v_scale[c];
+          }
           settle_scales(k_scale, v_scale);
         }
       };
@@ -600,7 +603,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
         const int tok_in_tile = tid / p.group, head = tid % p.group;
         for (int t = 0; t < w.n_tiles; ++t) {
           const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
-          const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
+          const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn &&
+                            B200_IN_BOUNDS(p.errs, w.it.seq.q0 + tok, 1, p.seqs.total_q, 140);
           const __nv_bfloat16* src = p.q + (long long)(w.it.seq.q0 + tok) * p.q_stride_t +
                                      (long long)(w.it.kvh * p.group + head) * p.q_stride_h;
           uint4 x[HD / 8];
@@ -711,7 +715,8 @@ __global__ void __launch_bounds__(ChunkCfg<FMT, HD>::THREADS, 1)
       const int j0 = w.j0, j1 = w.j1;
       if (t < w.n_tiles) {
         const int tok = w.it.rt * shape.tile_tokens + t * tile_tokens + tok_in_tile;
-        const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn;
+        const bool live = tok_in_tile < tile_tokens && tok < w.it.seq.qn &&
+                          B200_IN_BOUNDS(p.errs, w.it.seq.q0 + tok, 1, p.seqs.total_q, 143);
         const int lim = live ? w.it.seq.len - w.it.seq.qn + tok + 1 : 0;  // tokens that this row sees
         float m_used = -INFINITY, l = 0.f;
         float q_power = 1.f;
@@ -931,6 +936,7 @@ __global__ void __launch_bounds__(kItemRows)
   const int tok_in_tile = (row & 127) / p.group, head = (row & 127) % p.group;
   const int tok = rec.rt * shape.tile_tokens + (row >> 7) * tile_tokens + tok_in_tile;
   if (tok_in_tile >= tile_tokens || tok >= seq.qn) return;
+  if (!B200_IN_BOUNDS(p.errs, seq.q0 + tok, 1, p.seqs.total_q, 144)) return;
   float mx = -INFINITY;
   for (int i = 0; i < parts; ++i) {
     const int slot = join.slot(i);
@@ -1014,6 +1020,7 @@ __global__ void __launch_bounds__(128) paged_expand_kernel(PagedAttnParams p, Ex
       cell = ((page * p.pool.kv_heads + kvh) << p.seqs.page_log2) + (t & ((1 << p.seqs.page_log2) - 1));
     else
       report_error(p.errs, kErrBadIndex, b);
+    if (cell >= 0 && !B200_IN_BOUNDS(p.errs, cell, 1, pool_cells(p.seqs, p.pool.kv_heads), 145)) cell = -1;
   }
   float ks = cell >= 0 ? p.pool.k_scale[cell] : 0.f, vs = cell >= 0 ? p.pool.v_scale[cell] : 0.f;
   settle_scales(ks, vs);
