@@ -8,6 +8,7 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <vector>
 
@@ -25,6 +26,15 @@ std::string shape(const Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i) s += (i > 0 ? ", " : "") + std::to_string(t.size(i));
   return s + "]";
 }
+
+// These operators have no backward pass: a result that a gradient would be wanted through is refused.
+void no_backward(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(t == nullptr || !t->requires_grad(), name,
+                " has no backward pass; call it under torch.no_grad() or on detached tensors");
+}
+const Tensor* given(const std::optional<Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 void check_device(const Tensor& t, const Tensor& first, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
@@ -145,6 +155,7 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 void kv_cache_write(const Tensor& k_pages, const Tensor& v_pages, const std::optional<Tensor>& k_scale,
                     const std::optional<Tensor>& v_scale, const Tensor& k, const Tensor& v, const Tensor& table,
                     const Tensor& lens, const std::optional<Tensor>& starts) {
+  no_backward("kv_cache_write", {&k, &v, &k_pages, &v_pages, given(k_scale), given(v_scale)});
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
   const RowStrides sk = check_rows(k, -1, pool.kv_heads, pool.head_dim, false, "k");
   const RowStrides sv = check_rows(v, k.size(0), pool.kv_heads, pool.head_dim, false, "v");
@@ -161,6 +172,7 @@ std::tuple<Tensor, Tensor> kv_cache_read(const Tensor& k_pages, const Tensor& v_
                                          const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
                                          const Tensor& table, const Tensor& lens, const std::optional<Tensor>& starts,
                                          int64_t total, at::ScalarType type) {
+  no_backward("kv_cache_read", {&k_pages, &v_pages, given(k_scale), given(v_scale)});
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
   TORCH_CHECK(type == at::kBFloat16 || type == at::kFloat, "the cache is read as bfloat16 or float32");
   TORCH_CHECK(total >= 0, "total must not be negative");
@@ -178,6 +190,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                        const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
                        const std::optional<Tensor>& out_, const Tensor& table, const Tensor& lens,
                        const std::optional<Tensor>& starts, int64_t max_q, std::optional<double> scale_) {
+  no_backward("paged_attention", {&q, given(out_), &k_pages, &v_pages, given(k_scale), given(v_scale)});
   const b200::KvPool pool = check_pool(k_pages, v_pages, k_scale, v_scale);
   TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", shape(q));
   const int64_t heads = q.size(1);
@@ -290,6 +303,8 @@ Tensor adjust_logits(const Tensor& logits, const std::optional<Tensor>& out_, co
                      const std::optional<Tensor>& repetition, const std::optional<Tensor>& frequency,
                      const std::optional<Tensor>& presence, const std::optional<Tensor>& bias,
                      const std::optional<Tensor>& allowed) {
+  no_backward("adjust_logits",
+              {&logits, given(out_), given(repetition), given(frequency), given(presence), given(bias)});
   TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
               "logits must be [batch, vocab] with unit column stride");
   const int64_t batch = logits.size(0), vocab = logits.size(1);

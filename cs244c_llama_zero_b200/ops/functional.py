@@ -289,17 +289,11 @@ class KVPages(NamedTuple):
     v_scale: Optional[torch.Tensor] = None
 
 
-def _no_backward(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
-
-
 def kv_cache_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
                    kv_lens: torch.Tensor, q_starts: Optional[torch.Tensor] = None) -> None:
     """Write the new tokens' keys and values (bf16 ``[tokens, kv_heads, head_dim]``, any row strides that
     are multiples of 8) to their places in the cache, quantising them if the pages are 8-bit.  The pages
     that take new tokens must belong to one sequence each.  Rows of no sequence are ignored."""
-    _no_backward("kv_cache_write", k, v, *pages)
     _ext().kv_cache_write(*pages, k, v, block_table, kv_lens, q_starts)
 
 
@@ -309,7 +303,6 @@ def kv_cache_read(pages: KVPages, block_table: torch.Tensor, kv_lens: torch.Tens
     """The last tokens of every sequence out of the cache, as ``[total, kv_heads, head_dim]`` keys and
     values (bfloat16 or float32).  ``total`` is the number of rows (``q_starts[-1]``; default: one per
     sequence).  A row before its sequence's first token is zero; rows of no sequence are not written."""
-    _no_backward("kv_cache_read", *pages)
     if total is None:
         if q_starts is not None:
             raise ValueError("kv_cache_read: total (the number of rows) is needed with q_starts")
@@ -331,7 +324,6 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     see has no influence on it, whatever it is: tokens behind its position, the pages behind a sequence's end.
     An infinity or a NaN in a key that it does see makes it NaN, one in a value too (8-bit pages) or its column
     not finite (bf16)."""
-    _no_backward("paged_attention", q, out, *pages)
     if max_q_len is None:
         if q_starts is not None:
             raise ValueError("paged_attention: max_q_len is needed with q_starts")
@@ -356,7 +348,6 @@ def adjust_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     is added; tokens whose bit in ``allowed`` (int32 ``[ceil(vocab / 32)]`` or one row each, token t at bit
     ``t % 32`` of word ``t // 32``) is 0 become ``-inf``.  Computed in fp32.  ``out`` may be ``logits``.
     A token id outside the vocabulary is skipped and recorded (``ops.check_device_errors()``)."""
-    _no_backward("adjust_logits", logits, repetition_penalty, frequency_penalty, presence_penalty, bias, out)
     return _ext().adjust_logits(logits, out, history, history_lens, prompt_lens, repetition_penalty,
                                 frequency_penalty, presence_penalty, bias, allowed)
 
