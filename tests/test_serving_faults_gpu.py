@@ -236,3 +236,67 @@ def test_the_next_token_with_and_without_a_cache(hd, fmt):
     assert torch.equal(with_cache[:, :128], ids) and torch.equal(without[:, :128], ids)
     assert torch.equal(with_cache[clear, 128], without[clear, 128])
     assert torch.equal(without[clear, 128], want.argmax(-1)[clear])
+
+
+# ------------------------------------------------------------------------------------------ calls that the limits allow
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("group", [65, 100, 127, 128])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_the_largest_groups(F, fmt, group, hd):
+    """A tile holds one token's heads, and up to 63 rows of nothing."""
+    for q, kv in (([1, 1], [200, 33]), ([3, 0, 1], [150, 20, 128])):
+        b = Batch(q, kv, group, 1, hd, fmt, 16, seed=47)
+        _check(_attend(F, b), b)
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("q_lens", [[1, 2], [5, 33]])
+def test_thousands_of_sequences(F, fmt, q_lens):
+    """Far more sequences than threads that divide the work among them."""
+    b = Batch(q_lens, [40, 33], 8, 2, 64, fmt, 16, seed=48)
+    want = b.attention()
+    outs = _attend_many(F, b, copies=3000).double().cpu()
+    assert ((outs - want[0]).abs() <= bound(*want, fmt)).all()
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("max_q_len", [1, 4, 8, 30, 1000, 2 ** 31 - 1])
+def test_a_loose_bound_on_new_tokens(F, fmt, max_q_len):
+    """max_q_len chooses the form; any bound that holds gives the same result."""
+    b = Batch([1, 1, 1], [77, 300, 1], 8, 2, 128, fmt, 16, seed=49)
+    out = F.paged_attention(b.q.cuda(), b.pages("cuda"), b.table.cuda(), b.lens.cuda(), b.starts.cuda(), max_q_len)
+    _check(out, b)
+
+
+def test_logits_captured_and_on_two_streams(F):
+    """A captured call reads what its tensors hold at replay, in place too; two streams do not meet."""
+    gen = torch.Generator().manual_seed(50)
+    logits = torch.randn(3, 9001, generator=gen).cuda()
+    history = torch.randint(0, 9001, (3, 3000), generator=gen).cuda()
+    lens = torch.tensor([3000, 10, 0], dtype=torch.int32).cuda()
+    rep = torch.full((3,), 1.3).cuda()
+    want = F.adjust_logits(logits, history, lens, repetition_penalty=rep)
+    short = torch.tensor([5, 2900, 1], dtype=torch.int32).cuda()
+    want_short = F.adjust_logits(logits, history, short, repetition_penalty=rep)
+    torch.cuda.synchronize()
+    live, place = lens.clone(), logits.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.adjust_logits(logits, history, live, repetition_penalty=rep)
+        F.adjust_logits(place, history, live, repetition_penalty=rep, out=place)
+    graph.replay()
+    assert torch.equal(out, want) and torch.equal(place, want)
+    live.copy_(short)
+    place.copy_(logits)
+    graph.replay()
+    assert torch.equal(out, want_short) and torch.equal(place, want_short)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(10):
+        for s, n in zip(streams, (lens, short)):
+            with torch.cuda.stream(s):
+                results.append(F.adjust_logits(logits, history, n, repetition_penalty=rep))
+    torch.cuda.synchronize()
+    for i, r in enumerate(results):
+        assert torch.equal(r, want if i % 2 == 0 else want_short)
