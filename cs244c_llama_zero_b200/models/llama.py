@@ -371,7 +371,8 @@ class LlamaForCausalLM(nn.Module):
         ``input_ids`` [sum(rows)] holds ``rows[i]`` new tokens of cached sequence ``seqs[i]``, one sequence
         after the other: prompts, chunks of prompts or single tokens in any mixture.  Their keys and values
         are added to ``cache``; a step that is refused leaves its lengths and pages as they were.  ``weights``:
-        :meth:`decode_weights`, to lay them out once for many steps.
+        :meth:`decode_weights`, to lay them out once for many steps.  The blocks run by their weights, not through
+        their ``forward``: hooks on modules inside them do not fire.
         """
         from ..ops import functional as B
 

@@ -123,7 +123,7 @@ struct PagedAttnParams {
 // enqueued on the stream by this call; null where that much is not to be had and the caller can do without.
 using PagedAlloc = std::function<void*(size_t bytes, bool can_do_without)>;
 void paged_attention(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
-// Its form for more than 16 rows per kv head and sequence (paged_chunk.cu).
+// Its form for more than 64 rows per kv head and sequence, 32 for bf16 pages of head_dim 128 (paged_chunk.cu).
 void paged_attention_chunk(const PagedAttnParams& p, const PagedAlloc& alloc, cudaStream_t s);
 
 struct LogitsParams {

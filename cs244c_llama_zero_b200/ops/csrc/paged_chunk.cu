@@ -14,7 +14,7 @@
 //   3 (8-bit pages only): loads Q, and expands codes into the shared-memory tiles; see below.
 // With 8-bit pages the products are taken in fp16, whose 11 bits lose nothing next to the result's 8: a row of q is
 // scaled by a power of two to a maximum in [1, 2), and code * scale of K and of V by one for each unit of 128
-// tokens (to a maximum in (2^14, 2^15]); a token's factor and its product with a code are rounded there (2^-12
+// tokens (to a maximum in (2^14, 2^15]); a token's factor and its product with a code are rounded there (2^-11
 // relative each, for scales down to 2^-19 of the unit's largest).  K's power multiplies the unit's scores.  V's,
 // 2^e, goes into the exponent: the weights are 2^(s_j + e - m), with the running maximum m taken over s_j + e and
 // 2^6 of headroom, and the normaliser sums them times 2^-e.  Rounding code * scale to bf16 instead cost two bits of
@@ -24,11 +24,12 @@
 // powers of two beside them, and Q's rows, and the attention kernel loads both by TMA (KV_EXPANDED).
 // MMA order: S_A(0) S_B(0) | PV_A(j) S_A(j+1) PV_B(j) S_B(j+1) | ...
 //
-// Masking is by selection (a masked score becomes -inf whatever K holds).  A probability of 0 times an infinity or a NaN
-// is NaN, so V must hold none where some row of an item does not see it.  V's rows behind the last visible token
+// Masking is by selection (a masked score becomes -inf whatever K holds).  A probability of 0 times an infinity or a
+// NaN is NaN, so V must hold none where some row of an item does not see it.  V's rows behind the last visible token
 // are zeroed in shared memory: what lies in a page behind a sequence's end has no influence.  Infinities and NaN ahead
 // of it, in units that not all rows see whole, are zeroed too (bf16); a block that met some looks them up in the cache
-// once more in its epilogue, and writes NaN into the columns that held them for the rows that see them.
+// once more in its epilogue, and writes NaN into the columns that held them for the rows that see them (long chunk
+// 574 -> 580 us, ragged prompts 47 -> 49 us).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -136,7 +137,6 @@ __device__ __forceinline__ bool next_part_warp(ChunkWalk& w, const PagedSeqs& s,
   return more;
 }
 
-// 16 codes times a factor as 16 fp16.
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
   uint64_t r;
@@ -179,6 +179,7 @@ __device__ __forceinline__ void settle_scales(float& k, float& v) {
 // What a scale counts as in its unit's maximum: scales are not negative; infinities and NaN do not count.
 __device__ __forceinline__ uint32_t scale_bits(float x) { return x - x == 0.f ? __float_as_uint(x) : 0u; }
 
+// 16 codes times a factor as 16 fp16.
 template <int FMT>
 __device__ __forceinline__ void expand16(const uint4& q, float factor, uint4 (&out)[2]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};

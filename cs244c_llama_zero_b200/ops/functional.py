@@ -272,7 +272,8 @@ class KVPages(NamedTuple):
     and head in ``k_scale`` / ``v_scale`` ``[n_pages, kv_heads, page_size]`` (contiguous; pages and scales
     start on 16-byte boundaries): a row ``x`` is stored as
     ``scale = max|x| / M`` and ``code = round(x * M / max|x|)`` with M = 448 (e4m3) or 127 (int8).  A row
-    with an infinity or a NaN gets the scale NaN and reads back as NaN.  Scales are never negative.
+    with an infinity or a NaN gets the scale NaN and reads back as NaN.  Scales are never negative; attention
+    may take a ``v_scale`` below 2^-100 as 2^-100.
 
     A batch of sequences over such pages is described by ``block_table`` (int32 ``[batch, pages]``: token t
     of sequence b lies in page ``block_table[b, t // page_size]``), ``kv_lens`` (int32 ``[batch]``: cached
