@@ -176,8 +176,8 @@ __device__ __forceinline__ void settle_scales(float& k, float& v) {
     v = 0.f;
   }
 }
-// What a scale counts as in its unit's maximum: scales are not negative; infinities and NaN do not count.
-__device__ __forceinline__ uint32_t scale_bits(float x) { return x - x == 0.f ? __float_as_uint(x) : 0u; }
+// What a scale counts as in its unit's maximum, which compares bits: infinities, NaN and -0 do not count.
+__device__ __forceinline__ uint32_t scale_bits(float x) { return x > 0.f && x - x == 0.f ? __float_as_uint(x) : 0u; }
 
 // 16 codes times a factor as 16 fp16.
 template <int FMT>

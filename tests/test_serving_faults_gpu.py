@@ -92,6 +92,17 @@ def test_units_whose_values_are_zero(F, fmt, heads, q_len, v_size):
 
 
 @pytest.mark.parametrize("fmt", QUANTISED)
+@pytest.mark.parametrize("heads,q_len", FORMS)
+def test_scales_of_minus_zero(F, fmt, heads, q_len):
+    """A row of zeros may have been stored with the scale -0."""
+    b = Batch([q_len], [q_len + 200], *heads, fmt, 16, seed=51)
+    for which in range(2):
+        at = b.table[0, 2 + which], slice(None), 3
+        b.pools[which][at], b.scales[which][at] = 0, -0.0
+    _check(_attend(F, b), b)
+
+
+@pytest.mark.parametrize("fmt", QUANTISED)
 def test_many_values_of_zero(F, fmt):
     """Tens of thousands of zero V in one block's range, ahead of others, with scores that rise by less than makes
     the running maximum follow: the sum of their weights stays in range.  (The sequences share their pages.)"""
